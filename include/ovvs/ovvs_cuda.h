@@ -124,6 +124,102 @@ OVVS_API ovvsStatus ovvsIvfFlatSearchDevice(ovvsResources_t res, ovvsIvfFlatInde
                                             int32_t nprobe, const uint8_t* d_bitset,
                                             int64_t* d_neighbors, float* d_distances);
 
+/* ---- rows of scores in GPU memory: drawing, routing, grouping --------------------------------- */
+
+/* The drawn and the trained counterparts of ovvsTopk, for scores that are already on the GPU: a
+   search's scores, a router's or a language model's logits. All pointers are device pointers on
+   the Resources' device, aligned to their element. Each call checks its arguments, enqueues its
+   kernel on `stream` (NULL = the default stream) and returns; it uses no workspace and takes no
+   lock, so calls may run at once and may be captured into CUDA graphs. The caller's current
+   device is left as it was. Not in the reference.
+
+   Order: larger scores first, equal ones (-0 equals +0) by lower column, as ovvsTopk with
+   `largest`. A score of -inf, and a NaN, is masked: never drawn, never chosen, no weight and no
+   gradient. Any other value, the type's lowest included, is an ordinary score; where a row holds
+   +inf, its softmax is shared by the columns that hold it. */
+
+typedef enum ovvsScoreType {
+  OVVS_SCORE_F32 = 0,
+  OVVS_SCORE_F16 = 1,
+  OVVS_SCORE_BF16 = 16
+} ovvsScoreType;
+
+/* Draws `draws` columns, with replacement, from each row of logits [rows x cols] (row stride
+   `ld` >= cols elements). With weights w_j = exp((x_j - max) / temperature) and the columns of a
+   row in order, the columns kept are the shortest of
+     top_k   the first top_k (off: top_k <= 0),
+     top_p   the fewest first columns whose weights reach top_p times the weight of the columns
+             that top_k keeps (off: top_p >= 1 or NaN; at least one column),
+     min_p   the columns with x_j >= max + temperature * ln(min_p), min_p at most 1 (off:
+             min_p <= 0 or NaN).
+   The draw for a uniform u in [0, 1) is the first column, by column number, at which the running
+   sum of kept weights is above u times their total (u outside [0, 1), or NaN, counts as the
+   nearest value inside, NaN as 0). A temperature that is not above 0 takes the first column in
+   order with probability 1. A row with every score masked gives id -1, probability 0, kept 0.
+   Weights and their sums are 64-bit integers, so that no sum rounds: a weight is a multiple of
+   2^-50 of the row's largest up to 4,096 columns, of 2^-45 at 131,072 (one bit fewer for every
+   doubling), and one that rounds to 0 is kept like the others but never drawn, not for u = 0
+   either.
+   d_temperature, d_top_k, d_top_p, d_min_p: [rows], each may be NULL (1, off, off, off).
+   d_uniforms [rows x draws]. d_ids [rows x draws]; d_probs [rows x draws] (may be NULL) gets the
+   weight of each drawn column over the total that was drawn from; d_kept [rows] (may be NULL)
+   the number of columns kept. cols up to 2^31 - 1. */
+OVVS_API ovvsStatus ovvsSampleRowsDevice(ovvsResources_t res, const void* d_logits, int32_t type,
+                                         int64_t rows, int64_t cols, int64_t ld,
+                                         const float* d_temperature, const int32_t* d_top_k,
+                                         const float* d_top_p, const float* d_min_p,
+                                         const float* d_uniforms, int64_t draws, int64_t* d_ids,
+                                         float* d_probs, int32_t* d_kept, void* stream);
+
+typedef enum ovvsRouteScore { OVVS_ROUTE_SOFTMAX = 0, OVVS_ROUTE_SIGMOID = 1 } ovvsRouteScore;
+
+/* A group's value: its best choice value, or the sum of its two best. */
+typedef enum ovvsRouteGroupRule {
+  OVVS_ROUTE_GROUP_MAX = 0,
+  OVVS_ROUTE_GROUP_TOP2 = 1
+} ovvsRouteGroupRule;
+
+/* Chooses k experts for every token from logits [tokens x experts] (row stride `ld`). The scores
+   s are the row's softmax or sigmoids. Experts are ordered by their logits without a bias, by
+   s + bias (in 64 bits) with one. With groups > 1 the experts form `groups` groups of
+   neighbours, of which the topk_groups with the best value stand (TOP2 sums s without a bias,
+   s + bias with one; a group with one expert left has that one's value). d_ids [tokens x k]
+   holds the chosen experts in order, -1 where none is left; d_weights [tokens x k] scale * s, or
+   with `renormalize` scale * s / (sum of the chosen s), which holds also where the scores
+   themselves would vanish. The bias takes no part in weights or scores. An expert whose bias is
+   -inf or NaN is not chosen. d_scores [tokens x experts] (may be NULL) gets all s, 0 where
+   masked. At most 1024 experts, 32 groups, k <= 32 and k <= experts (SHAPE_MISMATCH beyond). */
+OVVS_API ovvsStatus ovvsRouteTopkDevice(ovvsResources_t res, const void* d_logits, int32_t type,
+                                        int64_t tokens, int64_t experts, int64_t ld,
+                                        const float* d_bias, int32_t score, int32_t groups,
+                                        int32_t topk_groups, int32_t group_rule, int32_t k,
+                                        int32_t renormalize, float scale, int32_t* d_ids,
+                                        float* d_weights, float* d_scores, void* stream);
+
+/* Gradient of ovvsRouteTopkDevice's weights, and of its scores where d_dscores is given, with
+   respect to the logits, for the same logits, score, renormalize and scale and the ids it chose
+   (entries outside [0, experts), and masked experts, have no part). d_dlogits [tokens x experts]
+   (the logits' type, row stride `ldd`) is written whole, 0 where masked; it may be the logits'
+   own memory with the same stride. The choice itself has no gradient, and neither has the bias.
+   At most 1024 experts, k <= 32. */
+OVVS_API ovvsStatus ovvsRouteTopkBackwardDevice(ovvsResources_t res, const void* d_logits,
+                                                int32_t type, int64_t tokens, int64_t experts,
+                                                int64_t ld, const int32_t* d_ids, int32_t k,
+                                                int32_t score, int32_t renormalize, float scale,
+                                                const float* d_dweights, const float* d_dscores,
+                                                void* d_dlogits, int64_t ldd, void* stream);
+
+/* Groups the pairs of d_ids [pairs] (a routed [tokens x k] array, flat) by expert, in pair order
+   within an expert, each expert's segment padded to a multiple of `align` places. d_offsets
+   [experts + 1]: the segments' starts, and the end of the last. d_order [capacity]: the pair that
+   stands at each place, -1 at padding and behind the last segment; capacity has to be at least
+   pairs + min(experts, pairs) * (align - 1) (SHAPE_MISMATCH below). d_position [pairs]: the place
+   of each pair, -1 where its id is outside [0, experts). At most 1024 experts. */
+OVVS_API ovvsStatus ovvsRoutePlanDevice(ovvsResources_t res, const int32_t* d_ids, int64_t pairs,
+                                        int64_t experts, int32_t align, int32_t* d_offsets,
+                                        int32_t* d_order, int64_t capacity, int32_t* d_position,
+                                        void* stream);
+
 /* ---- one process per GPU ------------------------------------------------------------------ */
 
 /* Size in bytes of the NCCL unique id that ovvsNcclUniqueId writes (128). */

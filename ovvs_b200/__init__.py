@@ -21,7 +21,7 @@ import numpy as np
 __all__ = [
     "OvvsError", "Resources", "BruteIndex", "IvfFlatIndex", "KMeans", "Batcher", "neighbors",
     "bitset_from_allow_list", "version", "library_path", "nccl_unique_id",
-    "METRIC", "DTYPE", "POLICY", "STATUS",
+    "METRIC", "DTYPE", "POLICY", "STATUS", "SCORE_TYPE", "ROUTE_SCORE", "ROUTE_GROUP_RULE",
 ]
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -33,6 +33,9 @@ POLICY = {"auto": 0, "npu_if_faster": 1, "gpu_if_faster": 2, "hetero": 3, "force
           "force_gpu": 5, "force_cpu": 6}
 STATUS = {0: "success", 1: "error", 2: "invalid argument", 3: "unsupported", 4: "out of memory",
           5: "compile fail", 6: "shape mismatch", 7: "device unavailable", 8: "io error"}
+SCORE_TYPE = {"float32": 0, "float16": 1, "bfloat16": 16}
+ROUTE_SCORE = {"softmax": 0, "sigmoid": 1}
+ROUTE_GROUP_RULE = {"max": 0, "top2": 1}
 _NP_DTYPE = {np.dtype(np.float32): "f32", np.dtype(np.float16): "f16", np.dtype(np.int8): "i8",
              np.dtype(np.uint8): "u8"}
 
@@ -105,6 +108,17 @@ def _bind(lib):
         # extensions (include/ovvs/ovvs_cuda.h)
         "ovvsIvfFlatSearchDevice": ([c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int32,
                                      c_void_p, c_void_p, c_void_p], c_int32),
+        "ovvsSampleRowsDevice": ([c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
+                                  c_void_p, c_void_p, c_void_p], c_int32),
+        "ovvsRouteTopkDevice": ([c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p,
+                                 c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_float,
+                                 c_void_p, c_void_p, c_void_p, c_void_p], c_int32),
+        "ovvsRouteTopkBackwardDevice": ([c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64,
+                                         c_void_p, c_int32, c_int32, c_int32, c_float, c_void_p,
+                                         c_void_p, c_void_p, c_int64, c_void_p], c_int32),
+        "ovvsRoutePlanDevice": ([c_void_p, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_void_p,
+                                 c_int64, c_void_p, c_void_p], c_int32),
         "ovvsResourcesStream": ([c_void_p, P(c_void_p)], c_int32),
         "ovvsResourcesSynchronize": ([c_void_p], c_int32),
         "ovvsResourcesDevice": ([c_void_p, P(c_int32)], c_int32),
@@ -169,12 +183,17 @@ def _dev_ptr(t) -> c_void_p:
     return c_void_p(int(t))
 
 
+def _type_name(t) -> str:
+    return str(t.dtype).rsplit(".", 1)[-1]
+
+
 class Resources:
     """One CUDA device + stream (reference: ovvsResources_t). ``device`` defaults to
     OVVS_CUDA_DEVICE or 0."""
 
     def __init__(self, _handle=None):
         self._h = c_void_p()
+        self._device = None
         if _handle is not None:
             self._h = _handle
         else:
@@ -329,6 +348,125 @@ class Resources:
         _check(lib().ovvsAllNeighbors(self._h, _ptr(a), a.shape[0], a.shape[1], m, int(k),
                                       _ptr(nb), _ptr(ds)), "all neighbors")
         return nb, ds
+
+    # Rows of scores on the GPU (include/ovvs/ovvs_cuda.h). The arguments are CUDA tensors
+    # (objects with data_ptr(), shape, stride(), dtype and device, e.g. torch's); outputs are
+    # written in place. Work is enqueued on `stream` (a cudaStream_t as an integer; None: this
+    # Resources' own stream, 0: the default stream) and not waited for.
+    def _device_scores(self, t, what):
+        """(pointer, score type, rows, cols, row stride) of a 2-D tensor of scores."""
+        type_ = SCORE_TYPE.get(_type_name(t))
+        if type_ is None:
+            raise ValueError(f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
+        if len(t.shape) != 2:
+            raise ValueError(f"{what} must be 2-D, not {tuple(t.shape)}")
+        rows, cols = t.shape
+        stride = t.stride()
+        if cols > 1 and stride[1] != 1:
+            raise ValueError(f"{what} must have neighbouring columns next to each other")
+        if rows > 1 and stride[0] < cols:
+            raise ValueError(f"{what} must not have overlapping rows")
+        return self._on_device(t, what), type_, rows, cols, stride[0] if rows > 1 else cols
+
+    def _on_device(self, t, what):
+        if self._device is None:
+            self._device = self.device()
+        d = t.device
+        if d.type != "cuda" or d.index != self._device:
+            raise ValueError(f"{what} is on {d}, not on cuda:{self._device}")
+        return t.data_ptr()
+
+    def _device_array(self, t, what, type_, shape):
+        """Pointer of a contiguous tensor of the given type and shape (None: null)."""
+        if t is None:
+            return None
+        if _type_name(t) != type_:
+            raise ValueError(f"{what} must be {type_}, not {t.dtype}")
+        if tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{what} must be contiguous {shape}, not {tuple(t.shape)}")
+        return self._on_device(t, what)
+
+    def _stream_of(self, stream):
+        return self.stream() if stream is None else int(stream)
+
+    def sample_rows(self, logits, uniforms, ids, probs=None, kept=None, temperature=None,
+                    top_k=None, top_p=None, min_p=None, stream=None):
+        """Draws from each row of logits [rows, cols] (ovvsSampleRowsDevice): for every uniform of
+        [rows] or [rows, draws] (f32 in [0, 1)) the drawn column into ids (i64) and its
+        probability among the kept columns into probs (f32), both shaped like uniforms, and the
+        number of kept columns into kept [rows] (i32). temperature, top_p, min_p (f32) and top_k
+        (i32) are [rows]; None leaves them off."""
+        lp, type_, rows, cols, ld = self._device_scores(logits, "logits")
+        shape = tuple(uniforms.shape)
+        if len(shape) not in (1, 2) or shape[0] != rows:
+            raise ValueError(f"uniforms must be [rows] or [rows, draws], not {shape}")
+        arr = self._device_array
+        per_row = (rows,)
+        _check(lib().ovvsSampleRowsDevice(
+            self._h, lp, type_, rows, cols, ld,
+            arr(temperature, "temperature", "float32", per_row),
+            arr(top_k, "top_k", "int32", per_row), arr(top_p, "top_p", "float32", per_row),
+            arr(min_p, "min_p", "float32", per_row), arr(uniforms, "uniforms", "float32", shape),
+            shape[1] if len(shape) == 2 else 1, arr(ids, "ids", "int64", shape),
+            arr(probs, "probs", "float32", shape), arr(kept, "kept", "int32", per_row),
+            self._stream_of(stream)), "sample rows")
+
+    def route_topk(self, logits, ids, weights, bias=None, score="softmax", groups=1,
+                   topk_groups=1, group_rule="max", renormalize=True, scale=1.0, scores=None,
+                   stream=None):
+        """The k experts of every token of logits [tokens, experts] (ovvsRouteTopkDevice) into
+        ids [tokens, k] (i32, -1 where none is left) and weights [tokens, k] (f32), and all scores
+        into scores [tokens, experts] (f32) where given. bias [experts] (f32) moves the choice,
+        not the weights."""
+        lp, type_, tokens, experts, ld = self._device_scores(logits, "logits")
+        if len(ids.shape) != 2 or ids.shape[0] != tokens:
+            raise ValueError(f"ids must be [tokens, k], not {tuple(ids.shape)}")
+        shape = tuple(ids.shape)
+        arr = self._device_array
+        _check(lib().ovvsRouteTopkDevice(
+            self._h, lp, type_, tokens, experts, ld, arr(bias, "bias", "float32", (experts,)),
+            ROUTE_SCORE[score], groups, topk_groups, ROUTE_GROUP_RULE[group_rule], shape[1],
+            bool(renormalize), scale, arr(ids, "ids", "int32", shape),
+            arr(weights, "weights", "float32", shape),
+            arr(scores, "scores", "float32", (tokens, experts)), self._stream_of(stream)),
+            "route top-k")
+
+    def route_topk_backward(self, logits, ids, dweights, dlogits, score="softmax",
+                            renormalize=True, scale=1.0, dscores=None, stream=None):
+        """Gradient of route_topk's weights (dweights [tokens, k] f32), and of its scores
+        (dscores [tokens, experts] f32) where given, with respect to the logits into dlogits
+        [tokens, experts] of the logits' type (ovvsRouteTopkBackwardDevice)."""
+        lp, type_, tokens, experts, ld = self._device_scores(logits, "logits")
+        dp, dtype, drows, dcols, ldd = self._device_scores(dlogits, "dlogits")
+        if (dtype, drows, dcols) != (type_, tokens, experts):
+            raise ValueError("dlogits must have the type and shape of the logits")
+        if len(ids.shape) != 2 or ids.shape[0] != tokens:
+            raise ValueError(f"ids must be [tokens, k], not {tuple(ids.shape)}")
+        shape = tuple(ids.shape)
+        arr = self._device_array
+        _check(lib().ovvsRouteTopkBackwardDevice(
+            self._h, lp, type_, tokens, experts, ld, arr(ids, "ids", "int32", shape), shape[1],
+            ROUTE_SCORE[score], bool(renormalize), scale,
+            arr(dweights, "dweights", "float32", shape),
+            arr(dscores, "dscores", "float32", (tokens, experts)), dp, ldd,
+            self._stream_of(stream)), "route top-k backward")
+
+    def route_plan(self, ids, experts, offsets, order, position, align=1, stream=None):
+        """Groups the pairs of ids [tokens, k] (i32) by expert (ovvsRoutePlanDevice): the starts
+        of the experts' segments, padded to multiples of `align`, into offsets [experts + 1], the
+        pair at each place into order [capacity] (-1 where none), capacity at least
+        ids.numel() + min(experts, ids.numel()) * (align - 1), and each pair's place into
+        position, shaped like ids (-1 for an id outside [0, experts)); all i32."""
+        shape = tuple(ids.shape)
+        pairs = 1
+        for n in shape:
+            pairs *= n
+        arr = self._device_array
+        _check(lib().ovvsRoutePlanDevice(
+            self._h, arr(ids, "ids", "int32", shape), pairs, experts, align,
+            arr(offsets, "offsets", "int32", (int(experts) + 1,)),
+            arr(order, "order", "int32", tuple(order.shape)), order.shape[0],
+            arr(position, "position", "int32", shape), self._stream_of(stream)), "route plan")
 
     def last_kernel_error(self) -> int:
         """Watchdog code seen by the last synchronising call that failed (0 if none); clears it."""

@@ -1,0 +1,81 @@
+// Operators over rows of scores that already live in GPU memory: drawing from a row, routing
+// tokens to experts with its gradient, and grouping the routed pairs by expert. They are the
+// drawn and the trained counterparts of the top-k selection in dense.cuh and keep its order:
+// larger scores first, equal ones (-0 == +0) by lower column.
+//
+// A score of -inf, and a NaN, is masked: it is never drawn or chosen and carries no weight or
+// gradient. Any other value, the type's lowest among them, is an ordinary score.
+//
+// No operator uses global workspace, so calls on several streams, or several captured graphs,
+// share nothing.
+#pragma once
+
+#include <cstdint>
+#include <cuda_runtime.h>
+
+namespace ovvs {
+namespace prim {
+
+// ovvsScoreType (ovvs_cuda.h).
+enum ScoreType : int { kScoreF32 = 0, kScoreF16 = 1, kScoreBf16 = 16 };
+
+struct SampleParams {
+  const void* logits;        // [rows x cols], row stride ld elements
+  int64_t rows, cols, ld;
+  const float* temperature;  // [rows] each, or null: 1, off, off, off
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  const float* uniforms;     // [rows x draws]
+  int64_t draws;
+  int64_t* ids;              // [rows x draws]
+  float* probs;              // [rows x draws] or null
+  int* kept;                 // [rows] or null
+};
+cudaError_t launch_sample_rows(const SampleParams& p, int type, cudaStream_t stream);
+
+constexpr int kRouteMaxExperts = 1024;
+constexpr int kRouteMaxK = 32;
+constexpr int kRouteMaxGroups = 32;
+
+struct RouteParams {
+  const void* logits;  // [tokens x experts], row stride ld elements
+  int64_t tokens, ld;
+  int experts;
+  const float* bias;   // [experts] or null
+  bool sigmoid;        // else softmax
+  int groups, topk_groups;
+  bool group_top2;     // else the group's best
+  int k;
+  bool renormalize;
+  float scale;
+  int* ids;            // [tokens x k]
+  float* weights;      // [tokens x k]
+  float* scores;       // [tokens x experts] or null
+};
+cudaError_t launch_route_topk(const RouteParams& p, int type, cudaStream_t stream);
+
+struct RouteBackwardParams {
+  const void* logits;
+  int64_t tokens, ld;
+  int experts;
+  const int* ids;         // [tokens x k]
+  int k;
+  bool sigmoid, renormalize;
+  float scale;
+  const float* dweights;  // [tokens x k]
+  const float* dscores;   // [tokens x experts] or null
+  void* dlogits;          // [tokens x experts], the logits' type, row stride ldd
+  int64_t ldd;
+};
+cudaError_t launch_route_topk_backward(const RouteBackwardParams& p, int type,
+                                       cudaStream_t stream);
+
+// Stable counting sort of pairs by expert. offsets [experts + 1]; order [capacity], -1 where no
+// pair stands; position [pairs], -1 for a pair whose id is outside [0, experts).
+cudaError_t launch_route_plan(const int* ids, int64_t pairs, int experts, int align,
+                              int* offsets, int* order, int64_t capacity, int* position,
+                              cudaStream_t stream);
+
+}  // namespace prim
+}  // namespace ovvs
