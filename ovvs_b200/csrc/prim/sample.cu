@@ -2,235 +2,718 @@
 //
 // Row x, temperature T, m = max x: weights w_j = exp((x_j - m) / T). Top-k, top-p and min-p each
 // keep a prefix of the row in top-k order (larger first, equal ones by lower column), so what is
-// kept is the shortest of the three and one (key, ties kept at that key) pair describes it. The
-// draw for a uniform u is the first column whose running sum of kept weights, in column order,
-// is above u times their total.
+// kept is the shortest of the three and ends at one (score, column), the edge. The draw for a
+// uniform u is the first column whose running sum of kept weights, in column order, is above u
+// times their total.
 //
 // Where a running sum crosses u * total, or p * total, must not hang on rounding or on the order
 // of an addition: neighbouring sums differ by one weight out of up to 2^31. So a weight is a
 // 64-bit integer, w_j * 2^frac rounded once, and every sum is an exact integer sum whatever its
 // order. frac = min(50, 62 - ceil(log2 cols)) leaves no sum above 2^63; weights below 2^-frac of
 // the row's largest (2^-45 at 131,072 columns) count as zero.
+//
+// One cluster of blocks takes one row. Each block holds its columns in shared memory, so the row
+// is read from HBM once and every later look at it costs shared memory only; what a block cannot
+// hold it reads again. Two ways lead from there:
+//   - top_k up to kDirectK, and greedy rows: the k-th largest of the threads' own maxima bounds
+//     the k-th score from below and lets little more than k columns pass. Those go to block 0,
+//     which orders and draws; the other blocks are done.
+//   - anything else: the edge of top-p is bracketed by a histogram of the weights over
+//     (m - x) / T, the few columns in the bracket are ordered by block 0, the weights above it
+//     are summed exactly. The draw walks the columns of the warp whose range of running sums
+//     holds it.
+// Where either meets more columns than its list holds (many equal or nearly equal scores), the
+// edge is found digit by digit of the score's bits.
 #include "rows.cuh"
+
+#include <cooperative_groups.h>
+
+#include <utility>
 
 #include "keys.cuh"
 #include "score_load.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace ovvs {
 namespace prim {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 256;
+constexpr int kMaxCluster = 8;
+constexpr int kList = 1024;     // columns block 0 can order
+constexpr int kRankList = 256;  // up to here it counts instead of sorting
+constexpr int kDirectK = 640;
+constexpr int kBins = 2048;
+constexpr float kBinsPerUnit = 64.f;  // histogram bins per unit of (m - x) / T
+static_assert(kBins * sizeof(float) == kList * sizeof(uint64_t), "the list holds the histogram");
+
+using u64 = unsigned long long;
 
 // Top-k order as an integer: larger is earlier; 0 marks a masked score.
 __device__ __forceinline__ uint32_t sort_key(float v) {
   return v > -INFINITY ? keys::order_bits(v) : 0u;
 }
 
-struct Row {
-  double m, rate;  // max; log2(e) / T
+// (score, column) in top-k order as one integer: larger is earlier.
+__device__ __forceinline__ u64 element(uint32_t key, uint32_t col) {
+  return (static_cast<u64>(key) << 32) | static_cast<uint32_t>(~col);
+}
+__device__ __forceinline__ uint32_t element_col(u64 e) { return ~static_cast<uint32_t>(e); }
+__device__ __forceinline__ uint32_t element_key(u64 e) { return static_cast<uint32_t>(e >> 32); }
+
+// 2^(i / 16), i < 16: one entry per pair of shared-memory banks.
+__constant__ double kSixteenths[16] = {
+    1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916,
+    1.189207115002721, 1.241857812073484, 1.2968395546510096, 1.3542555469368927,
+    1.4142135623730951, 1.4768261459394993, 1.5422108254079407, 1.6104903319492543,
+    1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+
+// Weights of one row. 2^(t / 16) = 2^(n >> 4) * 2^((n & 15) / 16) * 2^(f / 16) with n = round(t),
+// the last factor by its Taylor series in f * ln2 / 16 up to the fifth power: the sixth is at most
+// 1.4e-13. The result is rounded to an integer by adding 2^52.
+struct Weigher {
+  double m, rate;  // max; 16 log2(e) / T
+  float cut;       // scores below it weigh 0
+  bool top_inf;    // m is +inf: the columns that hold it weigh 1, the others 0
   int frac;
+  const double* table;
+
+  __device__ __forceinline__ void set(float max, float t, int frac_bits, const double* tab) {
+    frac = frac_bits;
+    table = tab;
+    top_inf = max == INFINITY;
+    m = top_inf ? 0.0 : max;
+    rate = 23.083120654223414 / static_cast<double>(t);
+    const double low = m - static_cast<double>(t) * 0.6931471805599453 * (frac + 1);
+    cut = top_inf ? INFINITY : fmaxf(__double2float_ru(low), -3.402823466e38f);
+  }
+  __device__ __forceinline__ u64 operator()(float x) const {
+    if (!(x >= cut)) return 0;
+    if (top_inf) return u64{1} << frac;
+    const double magic = 6755399441055744.0;  // 1.5 * 2^52
+    const double d = static_cast<double>(x) - m;
+    const double r = fma(d, rate, magic);
+    const int n = __double2loint(r);
+    const double f = fma(d, rate, magic - r);
+    double p = fma(f, 1.2715871950558131e-09, 1.467610032291943e-07);
+    p = fma(f, p, 1.3550807779497457e-05);
+    p = fma(f, p, 0.0009383847928089872);
+    p = fma(f, p, 0.04332169878499658);
+    p = fma(f, p, 1.0);
+    const double s = table[n & 15];
+    const double scaled = __hiloint2double(__double2hiint(s) + (frac + (n >> 4)) * (1 << 20),
+                                           __double2loint(s));
+    const double w = fma(p, scaled, 4503599627370496.0);
+    return static_cast<u64>(__double_as_longlong(w)) & ((u64{1} << 52) - 1);
+  }
 };
 
-__device__ __forceinline__ uint64_t weight(const Row& r, uint32_t key) {
-  const double x = keys::order_value(key);
-  const double d = x == r.m ? 0.0 : x - r.m;
-  const double a = d * r.rate;
-  if (!(a > -64.0)) return 0;
-  return static_cast<uint64_t>(__double2ll_rn(exp2(a + r.frac)));
+// 16 bytes of scores.
+template <class T>
+struct Chunk {
+  static constexpr int kN = 16 / sizeof(T);
+  static __device__ __forceinline__ uint4 masked();
+  static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[kN]);
+  // Largest of the chunk's scores that are not NaN; -inf without one.
+  static __device__ __forceinline__ float largest(const uint4& v) {
+    float x[kN];
+    unpack(v, x);
+    float m = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < kN; ++e) m = fmaxf(m, x[e]);
+    return m;
+  }
+};
+template <>
+__device__ __forceinline__ uint4 Chunk<float>::masked() {
+  return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
+}
+template <>
+__device__ __forceinline__ uint4 Chunk<__half>::masked() {
+  return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
+}
+template <>
+__device__ __forceinline__ uint4 Chunk<__nv_bfloat16>::masked() {
+  return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+}
+template <>
+__device__ __forceinline__ void Chunk<float>::unpack(const uint4& v, float (&x)[4]) {
+  x[0] = __uint_as_float(v.x);
+  x[1] = __uint_as_float(v.y);
+  x[2] = __uint_as_float(v.z);
+  x[3] = __uint_as_float(v.w);
+}
+template <>
+__device__ __forceinline__ void Chunk<__half>::unpack(const uint4& v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&w[i]);
+    x[2 * i] = __low2float(h);
+    x[2 * i + 1] = __high2float(h);
+  }
+}
+template <>
+__device__ __forceinline__ void Chunk<__nv_bfloat16>::unpack(const uint4& v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
 }
 
+struct Shared {
+  u64 list[kList];     // candidates; the histogram's totals before there are any
+  u64 wts[kList];      // their weights; the histogram before there are any
+  u64 pre[kList];      // running sums; the threads' maxima before there are any
+  u64 tot[kMaxCluster * kWarps];  // kept weight of every warp of the cluster
+  u64 xch[2][kMaxCluster];        // cluster_sum
+  u64 red[kWarps];
+  double table[16];
+  u64 edge;            // what block 0 found out
+  u64 above;
+  int state;
+  unsigned list_n;
+  unsigned pick;
+  unsigned bracket[2];
+  unsigned first;
+  int found;
+  int cnt;
+};
+static_assert(sizeof(uint32_t) * kMaxCluster * kThreads == sizeof(u64) * kList, "maxima fit");
+
 template <class V, class Op>
-__device__ V block_reduce(V v, Op op, V* buf) {
+__device__ __forceinline__ V warp_reduce(V v, Op op) {
+#pragma unroll
   for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(~0u, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = buf[0];
-  for (int w = 1; w < kWarps; ++w) v = op(v, buf[w]);
   return v;
 }
 
-// A prefix of the row in top-k order: every score above `key`, and the first `ties` columns
-// whose score is at it.
-struct Edge {
-  uint32_t key;
-  int64_t ties;
+struct Add {
+  template <class V>
+  __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
 };
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p, int frac) {
-  __shared__ uint64_t red[kWarps];
-  __shared__ uint64_t hist[kBins];
-  __shared__ uint64_t warp_sum[kWarps];
-  __shared__ uint64_t pick_sum;
-  __shared__ uint32_t pick_bin;
-  __shared__ int64_t found;
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t cols = p.cols;
-  const T* x = static_cast<const T*>(p.logits) + row * p.ld;
-  auto key_at = [&](int64_t j) { return sort_key(score_f32(x[j])); };
-  auto add = [](uint64_t a, uint64_t b) { return a + b; };
-  auto larger = [](uint64_t a, uint64_t b) { return a > b ? a : b; };
+__device__ __forceinline__ u64 block_sum(u64 v, u64* red) {
+  v = warp_reduce(v, Add());
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) v += red[w];
+  return v;
+}
 
-  uint64_t best = 0, n = 0;
-  for (int64_t j = tid; j < cols; j += kThreads) {
-    const uint32_t k = key_at(j);
-    if (!k) continue;
-    ++n;
-    best = larger(best, (static_cast<uint64_t>(k) << 32) | static_cast<uint32_t>(~j));
+// Exclusive running sum over the block's threads; *total gets the sum.
+__device__ __forceinline__ u64 block_scan(u64 v, u64* red, u64* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  u64 s = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 y = __shfl_up_sync(~0u, s, o);
+    if (lane >= o) s += y;
   }
-  best = block_reduce(best, larger, red);
-  n = block_reduce(n, add, red);
-  const float t = p.temperature ? p.temperature[row] : 1.f;
-  if (n == 0 || !(t > 0.f)) {  // nothing to draw from, or the first in top-k order
-    for (int64_t d = tid; d < p.draws; d += kThreads) {
-      p.ids[row * p.draws + d] = n ? static_cast<int64_t>(~static_cast<uint32_t>(best)) : -1;
-      if (p.probs) p.probs[row * p.draws + d] = n ? 1.f : 0.f;
+  __syncthreads();
+  if (lane == 31) red[warp] = s;
+  __syncthreads();
+  u64 before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += red[w];
+    all += red[w];
+  }
+  *total = all;
+  return before + s - v;
+}
+
+// Descending bitonic sort of n (a power of two, at least 2) integers.
+__device__ void sort_list(u64* a, int n) {
+  for (int size = 2; size <= n; size <<= 1) {
+    for (int stride = size >> 1; stride; stride >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n / 2; i += kThreads) {
+        const int lo = 2 * i - (i & (stride - 1)), hi = lo + stride;
+        const u64 x = a[lo], y = a[hi];
+        if ((x < y) == ((lo & size) == 0)) {
+          a[lo] = y;
+          a[hi] = x;
+        }
+      }
     }
-    if (tid == 0 && p.kept) p.kept[row] = n ? 1 : 0;
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ u64 draw_target(float u, u64 z) {
+  u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
+  return static_cast<u64>(static_cast<double>(u) * static_cast<double>(z));
+}
+
+// The weight that a top-p prefix has to reach.
+__device__ __forceinline__ u64 top_p_target(float tp, u64 z) {
+  const double want = ceil(static_cast<double>(fmaxf(tp, 0.f)) * static_cast<double>(z));
+  const u64 t = want < 1.0 ? 1 : static_cast<u64>(want);
+  return t < z ? t : z;
+}
+
+// Settings of one row.
+struct Settings {
+  float t, tp;
+  int k;
+  uint32_t mp_key;  // min-p: keys from here on stay (0: off)
+};
+
+// Block 0: orders the n listed columns, which hold every column that can be kept, and draws.
+__device__ void finish_list(const SampleParams& p, int64_t row, int n, const Settings& o,
+                            const Weigher& w, Shared& sh) {
+  const int tid = threadIdx.x;
+  const bool p_on = o.tp < 1.f;
+  u64 z = 0;
+  int nd = 0;  // columns with a weight to draw
+  int kept = 0;
+  if (n <= kRankList) {
+    // Every thread counts what stands before its column: its rank, and the weight before it.
+    const u64 e = tid < n ? sh.list[tid] : 0;
+    const u64 own = tid < n ? w(keys::order_value(element_key(e))) : 0;
+    if (tid < n) sh.wts[tid] = own;
+    __syncthreads();
+    int rank = 0;
+    u64 before = 0;
+    for (int j = 0; j < n; ++j) {
+      const bool less = sh.list[j] > e;
+      rank += less;
+      before += less ? sh.wts[j] : 0;
+    }
+    const int n1 = o.k > 0 && o.k < n ? o.k : n;
+    bool keep = tid < n && rank < n1 && element_key(e) >= o.mp_key;
+    if (p_on) {
+      const u64 z1 = block_sum(tid < n && rank < n1 ? own : 0, sh.red);
+      keep = keep && before < top_p_target(o.tp, z1);
+    }
+    kept = __syncthreads_count(keep);
+    nd = __syncthreads_count(keep && own);
+    z = block_sum(keep ? own : 0, sh.red);
+    if (tid < n) sh.wts[tid] = keep ? own : 0;
+    __syncthreads();
+    int at = 0;
+    before = 0;
+    for (int j = 0; j < n; ++j) {
+      const bool earlier = static_cast<uint32_t>(sh.list[j]) > static_cast<uint32_t>(e);
+      const u64 wj = sh.wts[j];
+      at += earlier && wj;
+      before += earlier ? wj : 0;
+    }
+    __syncthreads();
+    if (keep && own) {
+      sh.list[at] = (e << 32) | static_cast<unsigned>(tid);
+      sh.pre[at] = before;
+    }
+    __syncthreads();
+  } else {
+    const int n2 = n <= 512 ? 512 : kList;
+    for (int i = n + tid; i < n2; i += kThreads) sh.list[i] = 0;
+    sort_list(sh.list, n2);
+    const int per = n2 / kThreads, i0 = tid * per;
+    u64 sum = 0;
+    const int n1 = o.k > 0 && o.k < n ? o.k : n;
+    for (int i = i0; i < i0 + per; ++i) {
+      const u64 own = i < n1 ? w(keys::order_value(element_key(sh.list[i]))) : 0;
+      sh.wts[i] = own;
+      sum += own;
+    }
+    u64 z1;
+    u64 before = block_scan(sum, sh.red, &z1);
+    const u64 target = p_on ? top_p_target(o.tp, z1) : ~u64{0};
+    u64 part = 0;
+    int mine = 0, drawn = 0;
+    for (int i = i0; i < i0 + per; ++i) {
+      const u64 e = sh.list[i], own = sh.wts[i];
+      const bool keep = i < n1 && element_key(e) >= o.mp_key && before < target;
+      before += own;
+      mine += keep;
+      const bool draw = keep && own;
+      drawn += draw;
+      if (draw) part += own;
+      sh.list[i] = draw ? (e << 32) | static_cast<unsigned>(i) : 0;
+    }
+    kept = static_cast<int>(block_sum(mine, sh.red));
+    nd = static_cast<int>(block_sum(drawn, sh.red));
+    z = block_sum(part, sh.red);
+    sort_list(sh.list, n2);
+    sum = 0;
+    for (int i = i0; i < i0 + per && i < nd; ++i)
+      sum += sh.wts[static_cast<uint32_t>(sh.list[i])];
+    u64 all;
+    before = block_scan(sum, sh.red, &all);
+    for (int i = i0; i < i0 + per && i < nd; ++i) {
+      sh.pre[i] = before;
+      before += sh.wts[static_cast<uint32_t>(sh.list[i])];
+    }
+    __syncthreads();
+  }
+  if (tid == 0 && p.kept) p.kept[row] = kept;
+  for (int64_t d = tid; d < p.draws; d += kThreads) {
+    const u64 target = draw_target(p.uniforms[row * p.draws + d], z);
+    int lo = 0, hi = nd - 1;  // the last column whose running sum does not pass the target
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (sh.pre[mid] <= target)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    const u64 e = sh.list[lo];
+    p.ids[row * p.draws + d] = element_col(e >> 32);
+    if (p.probs)
+      p.probs[row * p.draws + d] = static_cast<float>(
+          static_cast<double>(sh.wts[static_cast<uint32_t>(e)]) / static_cast<double>(z));
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kThreads, 3)
+sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
+  using C = Chunk<T>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  Shared& sh = *reinterpret_cast<Shared*>(smem);
+  uint4* held = reinterpret_cast<uint4*>(smem + (sizeof(Shared) + 15) / 16 * 16);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int nb = static_cast<int>(cluster.num_blocks());
+  const int rank = static_cast<int>(cluster.block_rank());
+  const int64_t row = blockIdx.x / nb;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cols = static_cast<int>(p.cols);
+
+  // The row as 16-byte chunks on the boundaries of memory: chunk g holds columns g * kN - head
+  // and on. Each block, and in it each warp, takes a contiguous range of chunks.
+  const T* x = static_cast<const T*>(p.logits) + row * p.ld;
+  const int head = static_cast<int>((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % C::kN);
+  const uint4* base = reinterpret_cast<const uint4*>(x - head);
+  const int chunks = static_cast<int>((int64_t{cols} + head + C::kN - 1) / C::kN);
+  const int64_t b0 = int64_t{rank} * block_chunks;
+  const int local = static_cast<int>(
+      b0 < chunks ? (chunks - b0 < block_chunks ? chunks - b0 : block_chunks) : 0);
+  const int warp_chunks = (block_chunks + kWarps - 1) / kWarps;
+  const int c0 = warp * warp_chunks;
+  const int c1 = c0 + warp_chunks < local ? c0 + warp_chunks : local;
+  auto fetch = [&](int c) {  // from global memory; what lies outside the row is masked
+    const int64_t g = b0 + c;
+    const int64_t col = g * C::kN - head;
+    if (col >= 0 && col + C::kN <= cols) return __ldg(base + g);
+    uint4 v = C::masked();
+    T* lanes = reinterpret_cast<T*>(&v);
+#pragma unroll
+    for (int e = 0; e < C::kN; ++e)
+      if (col + e >= 0 && col + e < cols) lanes[e] = x[col + e];
+    return v;
+  };
+  auto chunk_at = [&](int c) { return c < resident ? held[c] : fetch(c); };
+  auto first_col = [&](int c) { return static_cast<int>((b0 + c) * C::kN - head); };
+
+  const float t = p.temperature ? p.temperature[row] : 1.f;
+  Settings o;
+  o.t = t;
+  o.tp = p.top_p ? p.top_p[row] : 1.f;
+  o.k = p.top_k ? p.top_k[row] : 0;
+  const float mp = p.min_p ? p.min_p[row] : 0.f;
+  const bool greedy = !(t > 0.f);
+
+  if (tid < 16) sh.table[tid] = kSixteenths[tid];
+  if (tid == 0) {
+    sh.list_n = 0;
+    sh.first = ~0u;
+  }
+  auto started = cluster.barrier_arrive();
+  float own = -INFINITY;
+#pragma unroll 4
+  for (int c = c0 + lane; c < c1; c += 32) {
+    const uint4 v = fetch(c);
+    if (c < resident) held[c] = v;
+    own = fmaxf(own, C::largest(v));
+  }
+
+  // Every thread's largest score, on every block.
+  uint32_t* maxima = reinterpret_cast<uint32_t*>(sh.pre);
+  const uint32_t own_key = sort_key(own);
+  cluster.barrier_wait(std::move(started));  // every block runs: its shared memory may be written
+  for (int b = 0; b < nb; ++b)
+    cluster.map_shared_rank(maxima, b)[rank * kThreads + tid] = own_key;
+  cluster.sync();
+  uint32_t top[kMaxCluster], best = 0;
+#pragma unroll
+  for (int b = 0; b < kMaxCluster; ++b) {
+    top[b] = b < nb ? maxima[b * kThreads + tid] : 0;
+    best = top[b] > best ? top[b] : best;
+  }
+  best = __reduce_max_sync(~0u, best);
+  if (lane == 0) sh.red[warp] = best;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    const uint32_t y = static_cast<uint32_t>(sh.red[i]);
+    best = y > best ? y : best;
+  }
+  if (best == 0) {  // every score is masked
+    if (rank == 0) {
+      for (int64_t d = tid; d < p.draws; d += kThreads) {
+        p.ids[row * p.draws + d] = -1;
+        if (p.probs) p.probs[row * p.draws + d] = 0.f;
+      }
+      if (tid == 0 && p.kept) p.kept[row] = 0;
+    }
     return;
   }
-  Row r;
-  r.m = keys::order_value(static_cast<uint32_t>(best >> 32));
-  r.rate = 1.4426950408889634074 / static_cast<double>(t);
-  r.frac = frac;
+  const float m = keys::order_value(best);
+  Shared* zero = cluster.map_shared_rank(&sh, 0);
 
-  // The last element of the shortest prefix of `in` whose sum of value(key) reaches `target`:
-  // one 8-bit digit of the key at a time, from the top.
-  auto reach = [&](Edge in, uint64_t target, auto value) {
-    uint64_t above = 0;
-    uint32_t prefix = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int b = tid; b < kBins; b += kThreads) hist[b] = 0;
-      __syncthreads();
-      const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
-      for (int64_t j = tid; j < cols; j += kThreads) {
-        const uint32_t k = key_at(j);
-        if (k > in.key && (k & mask) == prefix)
-          atomicAdd(reinterpret_cast<unsigned long long*>(&hist[(k >> shift) & 255]), value(k));
+  if (greedy) {  // the first column that holds the largest score
+    unsigned first = ~0u;
+    if (own_key == best) {
+      for (int c = c0 + lane; c < c1 && first == ~0u; c += 32) {
+        float v[C::kN];
+        C::unpack(chunk_at(c), v);
+#pragma unroll
+        for (int e = C::kN - 1; e >= 0; --e)
+          if (v[e] == m) first = static_cast<unsigned>(first_col(c) + e);
       }
-      if (tid == 0 && in.ties && (in.key & mask) == prefix)
-        atomicAdd(reinterpret_cast<unsigned long long*>(&hist[(in.key >> shift) & 255]),
-                  value(in.key) * in.ties);
-      __syncthreads();
-      if (tid == 0) {
-        uint64_t sum = above;
-        int b = kBins - 1;
-        while (b > 0 && sum + hist[b] < target) sum += hist[b--];
-        pick_bin = b;
-        pick_sum = sum;
+      atomicMin(&zero->first, first);
+    }
+    cluster.sync();
+    if (rank == 0) {
+      for (int64_t d = tid; d < p.draws; d += kThreads) {
+        p.ids[row * p.draws + d] = sh.first;
+        if (p.probs) p.probs[row * p.draws + d] = 1.f;
       }
-      __syncthreads();
-      prefix |= pick_bin << shift;
-      above = pick_sum;
+      if (tid == 0 && p.kept) p.kept[row] = 1;
     }
-    const uint64_t v = value(prefix);
-    return Edge{prefix, static_cast<int64_t>((target - above + v - 1) / v)};
-  };
-  auto tie_count = [&](uint32_t key) {
-    uint64_t c = 0;
-    for (int64_t j = tid; j < cols; j += kThreads) c += key_at(j) == key;
-    return static_cast<int64_t>(block_reduce(c, add, red));
-  };
-
-  Edge e{0, 0};
-  const int k = p.top_k ? p.top_k[row] : 0;
-  if (k > 0 && static_cast<uint64_t>(k) < n)
-    e = reach(e, static_cast<uint64_t>(k), [](uint32_t) { return uint64_t{1}; });
-  const float tp = p.top_p ? p.top_p[row] : 1.f;
-  if (tp < 1.f) {
-    uint64_t z = 0;
-    for (int64_t j = tid; j < cols; j += kThreads) {
-      const uint32_t kk = key_at(j);
-      if (kk > e.key) z += weight(r, kk);
-    }
-    z = block_reduce(z, add, red);
-    if (e.ties) z += weight(r, e.key) * e.ties;
-    const double want = ceil(static_cast<double>(fmaxf(tp, 0.f)) * static_cast<double>(z));
-    const uint64_t target = want < 1.0 ? 1 : static_cast<uint64_t>(want);
-    e = reach(e, target < z ? target : z, [&](uint32_t kk) { return weight(r, kk); });
+    return;
   }
-  const float mp = p.min_p ? p.min_p[row] : 0.f;
+
+  Weigher w;
+  w.set(m, t, frac, sh.table);
+  o.mp_key = 0;
   if (mp > 0.f) {
-    const double edge = r.m + static_cast<double>(t) * log(fmin(static_cast<double>(mp), 1.0));
-    const uint32_t ke = sort_key(__double2float_ru(edge));
-    if (ke > e.key) e = Edge{ke, INT64_MAX};
+    const double edge = static_cast<double>(m) +
+                        static_cast<double>(t) * log(fmin(static_cast<double>(mp), 1.0));
+    o.mp_key = sort_key(__double2float_ru(edge));
   }
-  uint64_t above = 0;
-  for (int64_t j = tid; j < cols; j += kThreads) above += key_at(j) > e.key;
-  above = block_reduce(above, add, red);
-  const int64_t have = e.key ? tie_count(e.key) : 0;
-  if (e.ties > have) e.ties = have;
-  if (tid == 0 && p.kept) p.kept[row] = static_cast<int>(above + e.ties);
 
-  // The column where the running sum of value(column, key) passes `target`: each warp sums a
-  // contiguous range, the owner of the target walks its range again.
-  const int64_t span = (cols + kThreads - 1) / kThreads * 32;
-  const int64_t j0 = warp * span, j1 = j0 + span < cols ? j0 + span : cols;
-  auto warp_totals = [&](auto value) {
-    uint64_t s = 0;
-    for (int64_t j = j0 + lane; j < j1; j += 32) s += value(j, key_at(j));
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-    __syncthreads();
-    if (lane == 0) warp_sum[warp] = s;
-    __syncthreads();
+  if (o.k > 0 && o.k <= kDirectK) {
+    // The largest bound found by halving that at least k maxima reach; every maximum is a score,
+    // so at least k scores reach it too.
+    // Every key is at least that of the type's lowest value, which lets all pass.
+    uint32_t lo = sort_key(-3.402823466e38f), hi = best;
+    for (int step = 0; step < 32 && lo < hi; ++step) {
+      const uint32_t mid = lo + (hi - lo + 1) / 2;
+      unsigned c = 0;
+#pragma unroll
+      for (int b = 0; b < kMaxCluster; ++b) c += top[b] >= mid;
+      c = __reduce_add_sync(~0u, c);
+      u64* buf = sh.tot + (step & 1) * kWarps;
+      if (lane == 0) buf[warp] = c;
+      __syncthreads();
+      c = 0;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) c += static_cast<unsigned>(buf[i]);
+      if (c >= static_cast<unsigned>(o.k)) {
+        lo = mid;
+        if (c <= static_cast<unsigned>(o.k + (o.k >> 3))) break;
+      } else {
+        hi = mid - 1;
+      }
+    }
+    const float bound = keys::order_value(lo);
+    for (int c = c0 + lane; c < c1; c += 32) {
+      const uint4 v = chunk_at(c);
+      if (!(C::largest(v) >= bound)) continue;
+      float y[C::kN];
+      C::unpack(v, y);
+#pragma unroll
+      for (int e = 0; e < C::kN; ++e) {
+        if (!(y[e] >= bound)) continue;
+        const unsigned at = atomicAdd(&zero->list_n, 1u);
+        if (at < kList) zero->list[at] = element(sort_key(y[e]), first_col(c) + e);
+      }
+    }
+    cluster.sync();
+    const unsigned n = zero->list_n;
+    if (n <= kList) {
+      if (nb > 1) cluster.sync();  // block 0's count has been read
+      if (rank == 0) finish_list(p, row, static_cast<int>(n), o, w, sh);
+      return;
+    }
+  }
+
+  // ---- the general way ----
+  // Value of each column of this warp's range, in column order per lane.
+  auto each = [&](auto&& f) {
+    for (int c = c0 + lane; c < c1; c += 32) {
+      float y[C::kN];
+      C::unpack(chunk_at(c), y);
+      const int col = first_col(c);
+#pragma unroll
+      for (int e = 0; e < C::kN; ++e) f(y[e], col + e);
+    }
   };
-  auto walk = [&](uint64_t before, uint64_t target, auto value, auto then) {
-    for (int64_t j = j0; j < j1; j += 32) {
-      const uint64_t own = j + lane < j1 ? value(j + lane, key_at(j + lane)) : 0;
-      uint64_t s = own;
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t y = __shfl_up_sync(~0u, s, o);
-        if (lane >= o) s += y;
+  int turn = 0;
+  auto cluster_sum = [&](u64 v) {
+    v = block_sum(v, sh.red);
+    turn ^= 1;
+    if (tid < nb) cluster.map_shared_rank(&sh, tid)->xch[turn][rank] = v;
+    cluster.sync();
+    u64 s = 0;
+    for (int b = 0; b < nb; ++b) s += sh.xch[turn][b];
+    return s;
+  };
+  // Sum of value(x, col) of every warp, on every block.
+  auto warp_totals = [&](auto&& value) {
+    u64 s = 0;
+    each([&](float y, int col) { s += value(y, col); });
+    s = warp_reduce(s, Add());
+    cluster.sync();
+    if (lane < nb) cluster.map_shared_rank(&sh, lane)->tot[rank * kWarps + warp] = s;
+    cluster.sync();
+  };
+  // The column of this warp's range at which before + the running sum passes target.
+  auto walk = [&](u64 before, u64 target, auto&& value, auto&& then) {
+    for (int c = c0; c < c1; c += 32) {
+      float y[C::kN];
+      u64 v[C::kN], sum = 0;
+      C::unpack(c + lane < c1 ? chunk_at(c + lane) : C::masked(), y);
+      const int col = first_col(c + lane);
+#pragma unroll
+      for (int e = 0; e < C::kN; ++e) {
+        v[e] = value(y[e], col + e);
+        sum += v[e];
+      }
+      u64 s = sum;
+#pragma unroll
+      for (int i = 1; i < 32; i <<= 1) {
+        const u64 z = __shfl_up_sync(~0u, s, i);
+        if (lane >= i) s += z;
       }
       const unsigned hit = __ballot_sync(~0u, before + s > target);
       if (hit) {
-        if (lane == __ffs(hit) - 1) then(j + lane, own);
+        if (lane == __ffs(hit) - 1) {
+          u64 run = before + s - sum;
+          bool done = false;
+#pragma unroll
+          for (int e = 0; e < C::kN; ++e) {
+            run += v[e];
+            if (!done && run > target) {
+              then(col + e, v[e]);
+              done = true;
+            }
+          }
+        }
         return;
       }
       before += __shfl_sync(~0u, s, 31);
     }
   };
-  int64_t last_tie = cols;  // columns of the ties that are kept end here
-  if (e.ties < have) {
-    auto is_tie = [&](int64_t, uint32_t kk) { return uint64_t{kk == e.key}; };
-    if (e.ties > 0) {
-      warp_totals(is_tie);
-      uint64_t before = 0;
-      for (int w = 0; w < warp; ++w) before += warp_sum[w];
-      const uint64_t target = static_cast<uint64_t>(e.ties) - 1;
-      if (target >= before && target < before + warp_sum[warp])
-        walk(before, target, is_tie, [&](int64_t j, uint64_t) { found = j; });
-      __syncthreads();
-      last_tie = found;
-    } else {
-      last_tie = -1;
+  auto before_warp = [&](u64* z) {
+    u64 before = 0, all = 0;
+    for (int i = 0; i < nb * kWarps; ++i) {
+      if (i == rank * kWarps + warp) before = all;
+      all += sh.tot[i];
     }
+    *z = all;
+    return before;
+  };
+  // Edge of the shortest prefix, among the columns up to `in`, whose sum of value(x) reaches
+  // target: the score one 8-bit digit at a time, then the column among those that share it.
+  auto reach = [&](u64 in, u64 target, auto&& value) {
+    u64* hist = sh.wts;
+    u64 above = 0;
+    uint32_t prefix = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      cluster.sync();
+      hist[tid] = 0;
+      __syncthreads();
+      const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
+      each([&](float y, int col) {
+        const uint32_t k = sort_key(y);
+        if (k && (k & mask) == prefix && element(k, col) >= in) {
+          const u64 v = value(y);
+          if (v) atomicAdd(&hist[(k >> shift) & 255], v);
+        }
+      });
+      cluster.sync();
+      u64 bin = 0, all;
+      for (int b = 0; b < nb; ++b) bin += cluster.map_shared_rank(hist, b)[255 - tid];
+      const u64 before = above + block_scan(bin, sh.red, &all);
+      if (before < target && before + bin >= target) {
+        sh.pick = 255 - tid;
+        sh.above = before;
+      }
+      __syncthreads();
+      prefix |= sh.pick << shift;
+      above = sh.above;
+    }
+    const u64 v = value(keys::order_value(prefix));
+    const u64 ties = (target - above + v - 1) / v;
+    auto tie = [&](float y, int col) {
+      const uint32_t k = sort_key(y);
+      return u64{k == prefix && element(k, col) >= in};
+    };
+    warp_totals(tie);
+    u64 all;
+    const u64 before = before_warp(&all);
+    if (ties - 1 >= before && ties - 1 < before + sh.tot[rank * kWarps + warp])
+      walk(before, ties - 1, tie, [&](int col, u64) {
+        for (int b = 0; b < nb; ++b) cluster.map_shared_rank(&sh, b)->found = col;
+      });
+    cluster.sync();
+    return element(prefix, static_cast<uint32_t>(sh.found));
+  };
+
+  u64 edge = element(1, ~0u);  // every column that is not masked
+  if (o.k > 0) {
+    u64 n = 0;
+    each([&](float y, int) { n += y > -INFINITY; });
+    n = cluster_sum(n);
+    if (static_cast<u64>(o.k) < n)
+      edge = reach(edge, static_cast<u64>(o.k), [](float) { return u64{1}; });
   }
-  auto kept_weight = [&](int64_t j, uint32_t kk) {
-    return kk > e.key || (kk && kk == e.key && j <= last_tie) ? weight(r, kk) : uint64_t{0};
+  if (o.tp < 1.f) {
+    u64 z = 0;
+    each([&](float y, int col) {
+      if (element(sort_key(y), col) >= edge) z += w(y);
+    });
+    z = cluster_sum(z);
+    edge = reach(edge, top_p_target(o.tp, z), [&](float y) { return w(y); });
+  }
+  if (o.mp_key > element_key(edge)) edge = element(o.mp_key, ~0u);
+  if (p.kept) {
+    u64 n = 0;
+    each([&](float y, int col) { n += element(sort_key(y), col) >= edge; });
+    n = cluster_sum(n);
+    if (rank == 0 && tid == 0) p.kept[row] = static_cast<int>(n);
+  }
+  auto kept_weight = [&](float y, int col) {
+    return element(sort_key(y), col) >= edge ? w(y) : u64{0};
   };
   warp_totals(kept_weight);
-  uint64_t z = 0, before = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w == warp) before = z;
-    z += warp_sum[w];
-  }
-  for (int64_t d = 0; d < p.draws; ++d) {
-    float u = p.uniforms[row * p.draws + d];
-    u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
-    const uint64_t target = static_cast<uint64_t>(static_cast<double>(u) * static_cast<double>(z));
-    if (target < before || target >= before + warp_sum[warp]) continue;
-    walk(before, target, kept_weight, [&](int64_t j, uint64_t own) {
-      p.ids[row * p.draws + d] = j;
-      if (p.probs)
-        p.probs[row * p.draws + d] =
-            static_cast<float>(static_cast<double>(own) / static_cast<double>(z));
-    });
+  u64 z;
+  const u64 before = before_warp(&z), mine = sh.tot[rank * kWarps + warp];
+  for (int64_t d0 = 0; d0 < p.draws; d0 += 32) {
+    const int64_t d = d0 + lane;
+    const u64 target = d < p.draws ? draw_target(p.uniforms[row * p.draws + d], z) : 0;
+    unsigned todo = __ballot_sync(~0u, d < p.draws && target >= before && target - before < mine);
+    while (todo) {
+      const int i = __ffs(todo) - 1;
+      todo &= todo - 1;
+      walk(before, __shfl_sync(~0u, target, i), kept_weight, [&](int col, u64 v) {
+        p.ids[row * p.draws + d0 + i] = col;
+        if (p.probs)
+          p.probs[row * p.draws + d0 + i] =
+              static_cast<float>(static_cast<double>(v) / static_cast<double>(z));
+      });
+    }
   }
 }
 
@@ -240,18 +723,40 @@ int frac_bits(int64_t cols) {
   return log2 < 12 ? 50 : 62 - log2;
 }
 
+template <class T>
+cudaError_t sample(const SampleParams& p, cudaStream_t stream) {
+  constexpr int kN = Chunk<T>::kN;
+  constexpr size_t kFixed = (sizeof(Shared) + 15) / 16 * 16;
+  const int64_t chunks = (p.cols + 2 * kN - 2) / kN;  // whatever the row's alignment
+  int nb = 1;
+  while (nb < kMaxCluster && chunks / nb > 512) nb *= 2;
+  const int block_chunks = static_cast<int>((chunks + nb - 1) / nb);
+  const int most = static_cast<int>((227 * 1024 - kFixed) / 16);
+  const int resident = block_chunks < most ? block_chunks : most;
+  const size_t smem = kFixed + static_cast<size_t>(resident) * 16;
+  cudaError_t e = cudaFuncSetAttribute(
+      sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.rows * nb));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(nb);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sample_kernel<T>, p, frac_bits(p.cols), block_chunks, resident);
+}
+
 }  // namespace
 
 cudaError_t launch_sample_rows(const SampleParams& p, int type, cudaStream_t stream) {
-  const unsigned grid = static_cast<unsigned>(p.rows);
-  const int frac = frac_bits(p.cols);
-  if (type == kScoreF32)
-    sample_kernel<float><<<grid, kThreads, 0, stream>>>(p, frac);
-  else if (type == kScoreF16)
-    sample_kernel<__half><<<grid, kThreads, 0, stream>>>(p, frac);
-  else
-    sample_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(p, frac);
-  return cudaGetLastError();
+  if (type == kScoreF32) return sample<float>(p, stream);
+  if (type == kScoreF16) return sample<__half>(p, stream);
+  return sample<__nv_bfloat16>(p, stream);
 }
 
 }  // namespace prim
