@@ -671,7 +671,8 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     return element(prefix, static_cast<uint32_t>(sh.found));
   };
 
-  u64 edge = element(1, ~0u);  // every column that is not masked
+  const u64 everything = element(1, ~0u);  // every column that is not masked
+  u64 edge = everything;
   if (o.k > 0) {
     u64 n = 0;
     each([&](float y, int) { n += y > -INFINITY; });
@@ -679,25 +680,162 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     if (static_cast<u64>(o.k) < n)
       edge = reach(edge, static_cast<u64>(o.k), [](float) { return u64{1}; });
   }
+  bool summed = false;  // tot holds the kept weights
   if (o.tp < 1.f) {
+    const bool limited = edge != everything;
+    const u64 in = edge;
+    auto inside = [&](float y, int col) { return !limited || element(sort_key(y), col) >= in; };
+    // Bins of (m - x) / T. A bin sums weights relative to its upper end, in 1 / unit, from a
+    // second-order series: good to 1e-5, which the bracket's margin covers. The edge's weight is
+    // at least (1 - p) / cols of the largest: bins beyond that are not needed.
+    const float per_unit = kBinsPerUnit / t;
+    const bool binned = !w.top_inf && per_unit > 0.f && per_unit < INFINITY;
+    const float unit = fminf(65536.f, 4294967040.f / (static_cast<float>(block_chunks) * C::kN));
+    const float reach_units = logf(static_cast<float>(cols) / (1.f - fmaxf(o.tp, 0.f)));
+    const int bins = min(kBins, static_cast<int>(reach_units * kBinsPerUnit) + 2);
+    unsigned* hist = reinterpret_cast<unsigned*>(sh.wts);
+    float* hist_total = reinterpret_cast<float*>(sh.list);
+    for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
+    __syncthreads();
     u64 z = 0;
     each([&](float y, int col) {
-      if (element(sort_key(y), col) >= edge) z += w(y);
+      if (!inside(y, col)) return;
+      z += w(y);
+      if (!binned) return;
+      const float v = (m - y) * per_unit;
+      if (!(v < static_cast<float>(bins))) return;
+      const int b = static_cast<int>(v);
+      const float f = (v - static_cast<float>(b)) * (1.f / kBinsPerUnit);
+      atomicAdd(&hist[b], static_cast<unsigned>(__float2int_rn(unit * (1.f - f * (1.f - 0.5f * f)))));
     });
     z = cluster_sum(z);
-    edge = reach(edge, top_p_target(o.tp, z), [&](float y) { return w(y); });
+    const u64 target = top_p_target(o.tp, z);
+    if (binned) {
+      const int share = kBins / nb;
+      for (int i = rank * share + tid; i < (rank + 1) * share; i += kThreads) {
+        float sum = 0.f;
+        for (int b = 0; b < nb; ++b)
+          sum += static_cast<float>(
+              cluster.map_shared_rank(reinterpret_cast<unsigned*>(sh.wts), b)[i]);
+        sum *= expf(-static_cast<float>(i) / kBinsPerUnit) / unit;
+        for (int b = 0; b < nb; ++b)
+          cluster.map_shared_rank(reinterpret_cast<float*>(sh.list), b)[i] = sum;
+      }
+      if (rank == 0 && tid == 0) {
+        sh.list_n = 0;
+        sh.cnt = 0;
+      }
+      if (tid == 0) {
+        sh.bracket[0] = sh.bracket[1] = static_cast<unsigned>(bins - 1);
+      }
+      cluster.sync();
+      // the bins where the running sum surely has not, and surely has, reached the target
+      constexpr int kPer = kBins / kThreads;
+      constexpr double kFix = 4294967296.0;
+      u64 part = 0, all;
+      for (int i = 0; i < kPer; ++i)
+        part += static_cast<u64>(hist_total[tid * kPer + i] * kFix);
+      u64 run = block_scan(part, sh.red, &all);
+      const double scale = exp2(static_cast<double>(-frac)) * kFix;
+      const double goal = static_cast<double>(target) * scale;
+      const double margin = 4e-5 * static_cast<double>(z) * scale;
+      for (int i = 0; i < kPer; ++i) {
+        const double lo = static_cast<double>(run);
+        run += static_cast<u64>(hist_total[tid * kPer + i] * kFix);
+        const double hi = static_cast<double>(run);
+        if (lo < goal - margin && hi >= goal - margin) sh.bracket[0] = tid * kPer + i;
+        if (lo < goal + margin && hi >= goal + margin) sh.bracket[1] = tid * kPer + i;
+      }
+      if (tid == 0 && !(goal - margin > 0.0)) sh.bracket[0] = 0;
+      __syncthreads();
+      const int first = static_cast<int>(sh.bracket[0]), last = static_cast<int>(sh.bracket[1]);
+      cluster.sync();  // no block looks at hist_total any more: the list may be written
+      u64 sum = 0;
+      int over = 0;
+      each([&](float y, int col) {
+        const float v = (m - y) * per_unit;
+        if (!(v < static_cast<float>(last + 1)) || !inside(y, col)) return;
+        if (v < static_cast<float>(first)) {
+          sum += w(y);
+          ++over;
+        } else {
+          const unsigned at = atomicAdd(&zero->list_n, 1u);
+          if (at < kList) zero->list[at] = element(sort_key(y), static_cast<uint32_t>(col));
+        }
+      });
+      sum = warp_reduce(sum, Add());
+      over = __reduce_add_sync(~0u, over);
+      if (lane == 0) {
+        zero->tot[rank * kWarps + warp] = sum;
+        atomicAdd(&zero->cnt, over);
+      }
+      cluster.sync();
+      if (rank == 0) {
+        const int n = static_cast<int>(sh.list_n);
+        u64 above = 0;
+        for (int i = 0; i < nb * kWarps; ++i) above += sh.tot[i];
+        __syncthreads();
+        if (tid == 0) sh.state = 0;
+        if (n > 0 && n <= kList && above < target) {
+          const int n2 = n <= 256 ? 256 : n <= 512 ? 512 : kList, per = n2 / kThreads;
+          for (int i = n + tid; i < n2; i += kThreads) sh.list[i] = 0;
+          sort_list(sh.list, n2);
+          u64 part2 = 0, all2;
+          for (int i = tid * per; i < (tid + 1) * per; ++i) {
+            sh.wts[i] = i < n ? w(keys::order_value(element_key(sh.list[i]))) : 0;
+            part2 += sh.wts[i];
+          }
+          u64 run2 = above + block_scan(part2, sh.red, &all2);
+          for (int i = tid * per; i < (tid + 1) * per; ++i) {
+            if (run2 >= target) break;
+            const u64 v = sh.wts[i];
+            if (i < n) {  // kept, whether or not it is the last
+              const int g = static_cast<int>((element_col(sh.list[i]) + static_cast<unsigned>(head))
+                                             / C::kN);
+              atomicAdd(&sh.tot[g / block_chunks * kWarps + g % block_chunks / warp_chunks], v);
+            }
+            run2 += v;
+            if (run2 >= target) {
+              sh.edge = sh.list[i];
+              sh.state = o.mp_key > element_key(sh.list[i]) ? 1 : 2;
+              sh.cnt += i + 1;
+            }
+          }
+        }
+        __syncthreads();
+        for (int b = 1; b < nb; ++b) {
+          Shared* peer = cluster.map_shared_rank(&sh, b);
+          if (tid < nb * kWarps) peer->tot[tid] = sh.tot[tid];
+          if (tid == 0) {
+            peer->edge = sh.edge;
+            peer->state = sh.state;
+          }
+        }
+      }
+      cluster.sync();
+      if (sh.state) edge = sh.edge;
+      summed = sh.state == 2;
+    }
+    if (!binned || sh.state == 0) edge = reach(in, target, [&](float y) { return w(y); });
   }
   if (o.mp_key > element_key(edge)) edge = element(o.mp_key, ~0u);
-  if (p.kept) {
-    u64 n = 0;
-    each([&](float y, int col) { n += element(sort_key(y), col) >= edge; });
-    n = cluster_sum(n);
-    if (rank == 0 && tid == 0) p.kept[row] = static_cast<int>(n);
-  }
   auto kept_weight = [&](float y, int col) {
     return element(sort_key(y), col) >= edge ? w(y) : u64{0};
   };
-  warp_totals(kept_weight);
+  if (!summed) {
+    u64 n = 0;
+    warp_totals([&](float y, int col) {
+      const bool keep = element(sort_key(y), col) >= edge;
+      n += keep;
+      return keep ? w(y) : u64{0};
+    });
+    if (p.kept) {
+      n = cluster_sum(n);
+      if (rank == 0 && tid == 0) p.kept[row] = static_cast<int>(n);
+    }
+  } else if (rank == 0 && tid == 0 && p.kept) {
+    p.kept[row] = sh.cnt;
+  }
   u64 z;
   const u64 before = before_warp(&z), mine = sh.tot[rank * kWarps + warp];
   for (int64_t d0 = 0; d0 < p.draws; d0 += 32) {
