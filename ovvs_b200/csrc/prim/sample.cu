@@ -28,6 +28,7 @@
 
 #include <cooperative_groups.h>
 
+#include <type_traits>
 #include <utility>
 
 #include "keys.cuh"
@@ -44,7 +45,9 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kList = 1024;     // columns block 0 can order
 constexpr int kRankList = 256;  // up to here it counts instead of sorting
-constexpr int kDirectK = 640;
+constexpr int kDirectK = 448;   // the largest top_k that the list serves
+constexpr int kRound = 8;       // chunks a thread has in flight where one block takes the row
+constexpr int kWanted = 520;    // columns it means to list
 constexpr int kBins = 2048;
 constexpr float kBinsPerUnit = 64.f;  // histogram bins per unit of (m - x) / T
 static_assert(kBins * sizeof(float) == kList * sizeof(uint64_t), "the list holds the histogram");
@@ -114,7 +117,17 @@ struct Weigher {
 template <class T>
 struct Chunk {
   static constexpr int kN = 16 / sizeof(T);
-  static __device__ __forceinline__ uint4 masked();
+  static constexpr uint32_t kMasked =  // -inf
+      sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;
+  static __device__ __forceinline__ uint32_t bits(float v) { return __float_as_uint(v); }
+  static __device__ __forceinline__ uint32_t bits(__half v) { return __half_as_ushort(v); }
+  static __device__ __forceinline__ uint32_t bits(__nv_bfloat16 v) {
+    return __bfloat16_as_ushort(v);
+  }
+  static __device__ __forceinline__ uint4 masked() {
+    const uint32_t w = sizeof(T) == 4 ? kMasked : kMasked << 16 | kMasked;
+    return make_uint4(w, w, w, w);
+  }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[kN]);
   // Largest of the chunk's scores that are not NaN; -inf without one.
   static __device__ __forceinline__ float largest(const uint4& v) {
@@ -126,18 +139,6 @@ struct Chunk {
     return m;
   }
 };
-template <>
-__device__ __forceinline__ uint4 Chunk<float>::masked() {
-  return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
-}
-template <>
-__device__ __forceinline__ uint4 Chunk<__half>::masked() {
-  return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
-}
-template <>
-__device__ __forceinline__ uint4 Chunk<__nv_bfloat16>::masked() {
-  return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
-}
 template <>
 __device__ __forceinline__ void Chunk<float>::unpack(const uint4& v, float (&x)[4]) {
   x[0] = __uint_as_float(v.x);
@@ -248,6 +249,97 @@ __device__ void sort_list(u64* a, int n) {
   __syncthreads();
 }
 
+// One warp: a bound that at least k of n keys reach, and, where the keys allow it, not many more;
+// the key of the type's lowest value, which every score reaches, when fewer than k do.
+__device__ uint32_t kth_bound(const uint32_t* key, int n, int k, uint32_t hi) {
+  const int lane = threadIdx.x & 31;
+  uint32_t lo = sort_key(-3.402823466e38f);
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo + 1) / 2;
+    int c = 0;
+    for (int i = lane; i < n; i += 32) c += key[i] >= mid;
+    c = __reduce_add_sync(~0u, c);
+    if (c >= k) {
+      lo = mid;
+      if (c <= k + (k >> 3)) break;
+    } else {
+      hi = mid - 1;
+    }
+  }
+  return lo;
+}
+
+// The same for the n listed columns, by the whole block; lo is a bound that k of them reach.
+__device__ uint32_t list_bound(Shared& sh, int n, int k, uint32_t lo) {
+  uint32_t own[kList / kThreads], hi = 0;
+#pragma unroll
+  for (int i = 0; i < kList / kThreads; ++i) {
+    const int at = i * kThreads + threadIdx.x;
+    own[i] = at < n ? element_key(sh.list[at]) : 0;
+    hi = max(hi, own[i]);
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto all = [&](unsigned v, u64* buf, auto op) {
+    if (lane == 0) buf[warp] = v;
+    __syncthreads();
+    unsigned r = static_cast<unsigned>(buf[0]);
+    for (int w = 1; w < kWarps; ++w) r = op(r, static_cast<unsigned>(buf[w]));
+    return r;
+  };
+  hi = all(__reduce_max_sync(~0u, hi), sh.red, [](unsigned a, unsigned b) { return max(a, b); });
+  for (int step = 0; lo < hi; ++step) {
+    const uint32_t mid = lo + (hi - lo + 1) / 2;
+    unsigned c = 0;
+#pragma unroll
+    for (int i = 0; i < kList / kThreads; ++i) c += own[i] >= mid;
+    c = all(__reduce_add_sync(~0u, c), sh.tot + (step & 1) * kWarps, Add());
+    if (c >= static_cast<unsigned>(k)) {
+      lo = mid;
+      if (c <= static_cast<unsigned>(k + (k >> 3))) break;
+    } else {
+      hi = mid - 1;
+    }
+  }
+  return lo;
+}
+
+// Keeps those of the first n listed columns whose key reaches lo; returns how many.
+__device__ unsigned keep_listed(Shared& sh, int n, uint32_t lo) {
+  u64 own[kList / kThreads];
+#pragma unroll
+  for (int i = 0; i < kList / kThreads; ++i) {
+    const int at = i * kThreads + threadIdx.x;
+    own[i] = at < n ? sh.list[at] : 0;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) sh.list_n = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kList / kThreads; ++i)
+    if (element_key(own[i]) >= lo) sh.list[atomicAdd(&sh.list_n, 1u)] = own[i];
+  __syncthreads();
+  const unsigned kept = sh.list_n;
+  __syncthreads();
+  return kept;
+}
+
+// Scores from here on pass min-p; 0 where it is off.
+__device__ __forceinline__ uint32_t min_p_key(float m, float t, float mp) {
+  if (!(mp > 0.f)) return 0;
+  const double edge = static_cast<double>(m) +
+                      static_cast<double>(t) * log(fmin(static_cast<double>(mp), 1.0));
+  return sort_key(__double2float_ru(edge));
+}
+
+// A row with every score masked.
+__device__ void nothing(const SampleParams& p, int64_t row) {
+  for (int64_t d = threadIdx.x; d < p.draws; d += kThreads) {
+    p.ids[row * p.draws + d] = -1;
+    if (p.probs) p.probs[row * p.draws + d] = 0.f;
+  }
+  if (threadIdx.x == 0 && p.kept) p.kept[row] = 0;
+}
+
 __device__ __forceinline__ u64 draw_target(float u, u64 z) {
   u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
   return static_cast<u64>(static_cast<double>(u) * static_cast<double>(z));
@@ -283,7 +375,9 @@ __device__ void finish_list(const SampleParams& p, int64_t row, int n, const Set
     __syncthreads();
     int rank = 0;
     u64 before = 0;
-    for (int j = 0; j < n; ++j) {
+    const int loops = (tid & ~31) < n ? n : 0;  // warps without a column have nothing to count
+#pragma unroll 4
+    for (int j = 0; j < loops; ++j) {
       const bool less = sh.list[j] > e;
       rank += less;
       before += less ? sh.wts[j] : 0;
@@ -301,7 +395,8 @@ __device__ void finish_list(const SampleParams& p, int64_t row, int n, const Set
     __syncthreads();
     int at = 0;
     before = 0;
-    for (int j = 0; j < n; ++j) {
+#pragma unroll 4
+    for (int j = 0; j < loops; ++j) {
       const bool earlier = static_cast<uint32_t>(sh.list[j]) > static_cast<uint32_t>(e);
       const u64 wj = sh.wts[j];
       at += earlier && wj;
@@ -375,7 +470,7 @@ __device__ void finish_list(const SampleParams& p, int64_t row, int n, const Set
 }
 
 template <class T>
-__global__ void __launch_bounds__(kThreads, 3)
+__global__ void __launch_bounds__(kThreads, 4)
 sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
   using C = Chunk<T>;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -400,16 +495,37 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
   const int warp_chunks = (block_chunks + kWarps - 1) / kWarps;
   const int c0 = warp * warp_chunks;
   const int c1 = c0 + warp_chunks < local ? c0 + warp_chunks : local;
-  auto fetch = [&](int c) {  // from global memory; what lies outside the row is masked
-    const int64_t g = b0 + c;
-    const int64_t col = g * C::kN - head;
-    if (col >= 0 && col + C::kN <= cols) return __ldg(base + g);
-    uint4 v = C::masked();
-    T* lanes = reinterpret_cast<T*>(&v);
+  // chunks of this block that lie in the row whole
+  const int whole0 = rank == 0 && head ? 1 : 0;
+  const bool cut_end = b0 + local == chunks && (static_cast<unsigned>(cols) + head) % C::kN;
+  const int whole = local - whole0 - (cut_end ? 1 : 0);
+  const uint4* here = base + b0;
+  auto cut = [&](int c) {  // a chunk at either end of the row: what lies outside is masked
+    const int64_t col = (b0 + c) * C::kN - head;
+    uint32_t bits[4] = {};
 #pragma unroll
-    for (int e = 0; e < C::kN; ++e)
-      if (col + e >= 0 && col + e < cols) lanes[e] = x[col + e];
-    return v;
+    for (int e = 0; e < C::kN; ++e) {
+      const bool in = col + e >= 0 && col + e < cols;
+      const uint32_t y = in ? C::bits(x[col + e]) : C::kMasked;
+      bits[e * 4 / C::kN] |= y << (e * sizeof(T) * 8 % 32);
+    }
+    return make_uint4(bits[0], bits[1], bits[2], bits[3]);
+  };
+  auto fetch = [&](int c) {  // from global memory
+    if (c - whole0 >= 0 && c - whole0 < whole) return __ldg(here + c);
+    return cut(c);
+  };
+  // kRound chunks at once, `step` apart; those from `end` on are masked
+  auto fetch_round = [&](uint4 (&v)[kRound], int c, int step, int end) {
+    const int last = c + (kRound - 1) * step;
+    if (__all_sync(~0u, c >= whole0 && last < whole0 + whole && last < end)) {
+#pragma unroll
+      for (int i = 0; i < kRound; ++i) v[i] = __ldg(here + c + i * step);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRound; ++i)
+        v[i] = c + i * step < end ? fetch(c + i * step) : C::masked();
+    }
   };
   auto chunk_at = [&](int c) { return c < resident ? held[c] : fetch(c); };
   auto first_col = [&](int c) { return static_cast<int>((b0 + c) * C::kN - head); };
@@ -428,43 +544,116 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     sh.first = ~0u;
   }
   auto started = cluster.barrier_arrive();
+  const bool direct = !greedy && o.k > 0 && o.k <= kDirectK;
+  if (direct && nb == 1) {
+    // One block for the row, nothing held. A look at every `skip`-th round of chunks, and the
+    // last, gives a bound: the k-th of all threads' two best chunks. Then every column that
+    // reaches it is listed, some k * skip of them; the rounds seen before come from L2.
+    __syncthreads();
+    uint32_t* maxima = reinterpret_cast<uint32_t*>(sh.pre);
+    const int skip = min(8, max(1, kWanted / o.k));
+    const int rounds = (local + kRound * kThreads - 1) / (kRound * kThreads);
+    uint4 v[kRound];
+    auto load_round = [&](int r) {
+      fetch_round(v, r * kRound * kThreads + tid, kThreads, local);
+    };
+    float big = -INFINITY, second = -INFINITY;
+    for (int r = 0; r < rounds; r = r + 1 < rounds ? min(r + skip, rounds - 1) : rounds) {
+      load_round(r);
+#pragma unroll
+      for (int i = 0; i < kRound; ++i) {
+        const float y = C::largest(v[i]);
+        second = fmaxf(second, fminf(big, y));
+        big = fmaxf(big, y);
+      }
+    }
+    maxima[tid] = sort_key(big);
+    maxima[kThreads + tid] = sort_key(second);
+    __syncthreads();
+    if (warp == 0) {
+      const uint32_t found = kth_bound(maxima, 2 * kThreads, o.k, ~0u);
+      if (lane == 0) sh.pick = found;
+    }
+    __syncthreads();
+    const float bound = keys::order_value(sh.pick);
+    for (int r = 0; r < rounds; ++r) {
+      load_round(r);
+#pragma unroll
+      for (int i = 0; i < kRound; ++i) {
+        if (!__ballot_sync(~0u, C::largest(v[i]) >= bound)) continue;
+        float y[C::kN];
+        C::unpack(v[i], y);
+        const int col = first_col((r * kRound + i) * kThreads + tid);
+#pragma unroll
+        for (int e = 0; e < C::kN; ++e) {
+          const bool pass = y[e] >= bound;
+          const unsigned who = __ballot_sync(~0u, pass);
+          if (!who) continue;
+          unsigned at = 0;
+          if (lane == __ffs(who) - 1) at = atomicAdd(&sh.list_n, __popc(who));
+          at = __shfl_sync(~0u, at, __ffs(who) - 1) + __popc(who & ((1u << lane) - 1));
+          if (pass && at < kList)
+            sh.list[at] = element(sort_key(y[e]), static_cast<uint32_t>(col + e));
+        }
+      }
+    }
+    __syncthreads();
+    unsigned listed = sh.list_n;
+    if (listed <= kList) {
+      if (listed > static_cast<unsigned>(o.k + o.k / 4)) {
+        const uint32_t lo = list_bound(sh, static_cast<int>(listed), o.k, sh.pick);
+        listed = keep_listed(sh, static_cast<int>(listed), lo);
+      }
+      uint32_t best = 0;
+      for (unsigned i = lane; i < listed; i += 32) best = max(best, element_key(sh.list[i]));
+      best = __reduce_max_sync(~0u, best);
+      if (best) {
+        Weigher w;
+        w.set(keys::order_value(best), t, frac, sh.table);
+        o.mp_key = min_p_key(keys::order_value(best), t, mp);
+        finish_list(p, row, static_cast<int>(listed), o, w, sh);
+      } else {
+        nothing(p, row);
+      }
+      return;
+    }
+    __syncthreads();
+    if (tid == 0) sh.list_n = 0;
+  }
   float own = -INFINITY;
-#pragma unroll 4
-  for (int c = c0 + lane; c < c1; c += 32) {
-    const uint4 v = fetch(c);
-    if (c < resident) held[c] = v;
-    own = fmaxf(own, C::largest(v));
+  for (int c = c0; c < c1; c += 32 * kRound) {
+    uint4 v[kRound];
+    fetch_round(v, c + lane, 32, c1);
+#pragma unroll
+    for (int i = 0; i < kRound; ++i) {
+      const int at = c + i * 32 + lane;
+      if (at < c1 && at < resident) held[at] = v[i];
+      own = fmaxf(own, C::largest(v[i]));
+    }
   }
 
-  // Every thread's largest score, on every block.
+  // The `heads` largest of each warp's threads' maxima, on every block.
   uint32_t* maxima = reinterpret_cast<uint32_t*>(sh.pre);
   const uint32_t own_key = sort_key(own);
+  const int heads = direct ? min(32, 1 + 2 * o.k / (nb * kWarps)) : 1;
   cluster.barrier_wait(std::move(started));  // every block runs: its shared memory may be written
-  for (int b = 0; b < nb; ++b)
-    cluster.map_shared_rank(maxima, b)[rank * kThreads + tid] = own_key;
-  cluster.sync();
-  uint32_t top[kMaxCluster], best = 0;
-#pragma unroll
-  for (int b = 0; b < kMaxCluster; ++b) {
-    top[b] = b < nb ? maxima[b * kThreads + tid] : 0;
-    best = top[b] > best ? top[b] : best;
-  }
-  best = __reduce_max_sync(~0u, best);
-  if (lane == 0) sh.red[warp] = best;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    const uint32_t y = static_cast<uint32_t>(sh.red[i]);
-    best = y > best ? y : best;
-  }
-  if (best == 0) {  // every score is masked
-    if (rank == 0) {
-      for (int64_t d = tid; d < p.draws; d += kThreads) {
-        p.ids[row * p.draws + d] = -1;
-        if (p.probs) p.probs[row * p.draws + d] = 0.f;
-      }
-      if (tid == 0 && p.kept) p.kept[row] = 0;
+  {
+    uint32_t left = own_key;
+    for (int i = 0; i < heads; ++i) {
+      const uint32_t big = __reduce_max_sync(~0u, left);
+      if (lane < nb)
+        cluster.map_shared_rank(maxima, lane)[(rank * kWarps + warp) * heads + i] = big;
+      const unsigned at = __ballot_sync(~0u, left == big);
+      if (lane == __ffs(at) - 1) left = 0;
     }
+  }
+  cluster.sync();
+  const int num_maxima = nb * kWarps * heads;
+  uint32_t best = 0;  // a warp's first is its largest
+  for (int i = lane; i < nb * kWarps; i += 32) best = max(best, maxima[i * heads]);
+  best = __reduce_max_sync(~0u, best);
+  if (best == 0) {  // every score is masked
+    if (rank == 0) nothing(p, row);
     return;
   }
   const float m = keys::order_value(best);
@@ -495,37 +684,17 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
 
   Weigher w;
   w.set(m, t, frac, sh.table);
-  o.mp_key = 0;
-  if (mp > 0.f) {
-    const double edge = static_cast<double>(m) +
-                        static_cast<double>(t) * log(fmin(static_cast<double>(mp), 1.0));
-    o.mp_key = sort_key(__double2float_ru(edge));
-  }
+  o.mp_key = min_p_key(m, t, mp);
 
-  if (o.k > 0 && o.k <= kDirectK) {
+  if (direct) {
     // The largest bound found by halving that at least k maxima reach; every maximum is a score,
     // so at least k scores reach it too.
-    // Every key is at least that of the type's lowest value, which lets all pass.
-    uint32_t lo = sort_key(-3.402823466e38f), hi = best;
-    for (int step = 0; step < 32 && lo < hi; ++step) {
-      const uint32_t mid = lo + (hi - lo + 1) / 2;
-      unsigned c = 0;
-#pragma unroll
-      for (int b = 0; b < kMaxCluster; ++b) c += top[b] >= mid;
-      c = __reduce_add_sync(~0u, c);
-      u64* buf = sh.tot + (step & 1) * kWarps;
-      if (lane == 0) buf[warp] = c;
-      __syncthreads();
-      c = 0;
-#pragma unroll
-      for (int i = 0; i < kWarps; ++i) c += static_cast<unsigned>(buf[i]);
-      if (c >= static_cast<unsigned>(o.k)) {
-        lo = mid;
-        if (c <= static_cast<unsigned>(o.k + (o.k >> 3))) break;
-      } else {
-        hi = mid - 1;
-      }
+    if (warp == 0) {
+      const uint32_t found = kth_bound(maxima, num_maxima, o.k, best);
+      if (lane == 0) sh.pick = found;
     }
+    __syncthreads();
+    const uint32_t lo = sh.pick;
     const float bound = keys::order_value(lo);
     for (int c = c0 + lane; c < c1; c += 32) {
       const uint4 v = chunk_at(c);
@@ -867,9 +1036,10 @@ cudaError_t sample(const SampleParams& p, cudaStream_t stream) {
   constexpr size_t kFixed = (sizeof(Shared) + 15) / 16 * 16;
   const int64_t chunks = (p.cols + 2 * kN - 2) / kN;  // whatever the row's alignment
   int nb = 1;
-  while (nb < kMaxCluster && chunks / nb > 512) nb *= 2;
+  const bool one_pass = p.top_k && p.rows >= 296;
+  while (nb < kMaxCluster && chunks / nb > 512 && !one_pass) nb *= 2;
   const int block_chunks = static_cast<int>((chunks + nb - 1) / nb);
-  const int most = static_cast<int>((227 * 1024 - kFixed) / 16);
+  const int most = static_cast<int>(((one_pass ? 56 : 227) * 1024 - kFixed) / 16);
   const int resident = block_chunks < most ? block_chunks : most;
   const size_t smem = kFixed + static_cast<size_t>(resident) * 16;
   cudaError_t e = cudaFuncSetAttribute(
