@@ -74,8 +74,9 @@ __constant__ double kSixteenths[16] = {
     1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
 
 // Weights of one row. 2^(t / 16) = 2^(n >> 4) * 2^((n & 15) / 16) * 2^(f / 16) with n = round(t),
-// the last factor by its Taylor series in f * ln2 / 16 up to the fifth power: the sixth is at most
-// 1.4e-13. The result is rounded to an integer by adding 2^52.
+// the last factor by the polynomial of degree 4 through its values at the Chebyshev points of
+// [-1/2, 1/2], which is 2^-38.5 off at most: ten 64-bit operations a weight, where the power
+// function takes some forty. The result is rounded to an integer by adding 2^52.
 struct Weigher {
   double m, rate;  // max; 16 log2(e) / T
   float cut;       // scores below it weigh 0
@@ -100,10 +101,9 @@ struct Weigher {
     const double r = fma(d, rate, magic);
     const int n = __double2loint(r);
     const double f = fma(d, rate, magic - r);
-    double p = fma(f, 1.2715871950558131e-09, 1.467610032291943e-07);
-    p = fma(f, p, 1.3550807779497457e-05);
-    p = fma(f, p, 0.0009383847928089872);
-    p = fma(f, p, 0.04332169878499658);
+    double p = fma(f, 1.4676387238435006e-07, 1.3551205154935067e-05);
+    p = fma(f, p, 0.0009383847926296646);
+    p = fma(f, p, 0.043321698760160544);
     p = fma(f, p, 1.0);
     const double s = table[n & 15];
     const double scaled = __hiloint2double(__double2hiint(s) + (frac + (n >> 4)) * (1 << 20),
@@ -174,6 +174,7 @@ struct Shared {
   u64 xch[2][kMaxCluster];        // cluster_sum
   u64 red[kWarps];
   double table[16];
+  float queue[kWarps][64];
   u64 edge;            // what block 0 found out
   u64 above;
   int state;
@@ -249,15 +250,31 @@ __device__ void sort_list(u64* a, int n) {
   __syncthreads();
 }
 
-// One warp: a bound that at least k of n keys reach, and, where the keys allow it, not many more;
-// the key of the type's lowest value, which every score reaches, when fewer than k do.
-__device__ uint32_t kth_bound(const uint32_t* key, int n, int k, uint32_t hi) {
+// One warp: a bound that at least k of n <= 32 * kPer keys reach, and, where the keys allow it,
+// not many more; the key of the type's lowest value, which every score reaches, when fewer than
+// k do.
+template <int kPer>
+__device__ uint32_t kth_bound(const uint32_t* key, int n, int k) {
   const int lane = threadIdx.x & 31;
-  uint32_t lo = sort_key(-3.402823466e38f);
+  uint32_t own[kPer], hi = 0, least = ~0u;
+  int valid = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    own[i] = i * 32 + lane < n ? key[i * 32 + lane] : 0;
+    hi = max(hi, own[i]);
+    if (own[i]) {
+      least = min(least, own[i]);
+      ++valid;
+    }
+  }
+  if (static_cast<int>(__reduce_add_sync(~0u, valid)) < k) return sort_key(-3.402823466e38f);
+  hi = __reduce_max_sync(~0u, hi);
+  uint32_t lo = __reduce_min_sync(~0u, least);
   while (lo < hi) {
     const uint32_t mid = lo + (hi - lo + 1) / 2;
     int c = 0;
-    for (int i = lane; i < n; i += 32) c += key[i] >= mid;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) c += own[i] >= mid;
     c = __reduce_add_sync(~0u, c);
     if (c >= k) {
       lo = mid;
@@ -368,43 +385,54 @@ __device__ void finish_list(const SampleParams& p, int64_t row, int n, const Set
   int nd = 0;  // columns with a weight to draw
   int kept = 0;
   if (n <= kRankList) {
-    // Every thread counts what stands before its column: its rank, and the weight before it.
-    const u64 e = tid < n ? sh.list[tid] : 0;
-    const u64 own = tid < n ? w(keys::order_value(element_key(e))) : 0;
-    if (tid < n) sh.wts[tid] = own;
+    // `share` threads count what stands before a column: its rank, and the weight before it.
+    const int share = n <= 32 ? 8 : n <= 64 ? 4 : n <= 128 ? 2 : 1;
+    const int i = tid / share, part = tid % share;
+    auto joined = [&](auto v) {
+      for (int s = 1; s < share; s <<= 1) v += __shfl_xor_sync(~0u, v, s);
+      return v;
+    };
+    const bool here = i < n, one = here && part == 0;
+    const u64 e = here ? sh.list[i] : 0;
+    const u64 own = here ? w(keys::order_value(element_key(e))) : 0;
+    if (one) sh.wts[i] = own;
     __syncthreads();
     int rank = 0;
     u64 before = 0;
-    const int loops = (tid & ~31) < n ? n : 0;  // warps without a column have nothing to count
+    const int loops = (tid & ~31) / share < n ? n : 0;  // not for a warp without a column
 #pragma unroll 4
-    for (int j = 0; j < loops; ++j) {
+    for (int j = part; j < loops; j += share) {
       const bool less = sh.list[j] > e;
       rank += less;
       before += less ? sh.wts[j] : 0;
     }
+    rank = joined(rank);
+    before = joined(before);
     const int n1 = o.k > 0 && o.k < n ? o.k : n;
-    bool keep = tid < n && rank < n1 && element_key(e) >= o.mp_key;
+    bool keep = here && rank < n1 && element_key(e) >= o.mp_key;
     if (p_on) {
-      const u64 z1 = block_sum(tid < n && rank < n1 ? own : 0, sh.red);
+      const u64 z1 = block_sum(one && rank < n1 ? own : 0, sh.red);
       keep = keep && before < top_p_target(o.tp, z1);
     }
-    kept = __syncthreads_count(keep);
-    nd = __syncthreads_count(keep && own);
-    z = block_sum(keep ? own : 0, sh.red);
-    if (tid < n) sh.wts[tid] = keep ? own : 0;
+    kept = __syncthreads_count(keep && one);
+    nd = __syncthreads_count(keep && one && own);
+    z = block_sum(keep && one ? own : 0, sh.red);
+    if (one) sh.wts[i] = keep ? own : 0;
     __syncthreads();
     int at = 0;
     before = 0;
 #pragma unroll 4
-    for (int j = 0; j < loops; ++j) {
+    for (int j = part; j < loops; j += share) {
       const bool earlier = static_cast<uint32_t>(sh.list[j]) > static_cast<uint32_t>(e);
       const u64 wj = sh.wts[j];
       at += earlier && wj;
       before += earlier ? wj : 0;
     }
+    at = joined(at);
+    before = joined(before);
     __syncthreads();
-    if (keep && own) {
-      sh.list[at] = (e << 32) | static_cast<unsigned>(tid);
+    if (keep && one && own) {
+      sh.list[at] = (e << 32) | static_cast<unsigned>(i);
       sh.pre[at] = before;
     }
     __syncthreads();
@@ -571,29 +599,44 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     maxima[kThreads + tid] = sort_key(second);
     __syncthreads();
     if (warp == 0) {
-      const uint32_t found = kth_bound(maxima, 2 * kThreads, o.k, ~0u);
+      const uint32_t found = kth_bound<2 * kThreads / 32>(maxima, 2 * kThreads, o.k);
       if (lane == 0) sh.pick = found;
     }
     __syncthreads();
     const float bound = keys::order_value(sh.pick);
     for (int r = 0; r < rounds; ++r) {
       load_round(r);
+      unsigned count = 0;
 #pragma unroll
       for (int i = 0; i < kRound; ++i) {
-        if (!__ballot_sync(~0u, C::largest(v[i]) >= bound)) continue;
+        if (!(C::largest(v[i]) >= bound)) continue;
+        float y[C::kN];
+        C::unpack(v[i], y);
+#pragma unroll
+        for (int e = 0; e < C::kN; ++e) count += y[e] >= bound;
+      }
+      if (!__ballot_sync(~0u, count)) continue;
+      unsigned at = count;  // places for the whole warp at once
+#pragma unroll
+      for (int i = 1; i < 32; i <<= 1) {
+        const unsigned y = __shfl_up_sync(~0u, at, i);
+        if (lane >= i) at += y;
+      }
+      unsigned base_at = 0;
+      if (lane == 31) base_at = atomicAdd(&sh.list_n, at);
+      at += __shfl_sync(~0u, base_at, 31) - count;
+      if (count == 0) continue;
+#pragma unroll
+      for (int i = 0; i < kRound; ++i) {
+        if (!(C::largest(v[i]) >= bound)) continue;
         float y[C::kN];
         C::unpack(v[i], y);
         const int col = first_col((r * kRound + i) * kThreads + tid);
 #pragma unroll
         for (int e = 0; e < C::kN; ++e) {
-          const bool pass = y[e] >= bound;
-          const unsigned who = __ballot_sync(~0u, pass);
-          if (!who) continue;
-          unsigned at = 0;
-          if (lane == __ffs(who) - 1) at = atomicAdd(&sh.list_n, __popc(who));
-          at = __shfl_sync(~0u, at, __ffs(who) - 1) + __popc(who & ((1u << lane) - 1));
-          if (pass && at < kList)
-            sh.list[at] = element(sort_key(y[e]), static_cast<uint32_t>(col + e));
+          if (!(y[e] >= bound)) continue;
+          if (at < kList) sh.list[at] = element(sort_key(y[e]), static_cast<uint32_t>(col + e));
+          ++at;
         }
       }
     }
@@ -635,7 +678,7 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
   // The `heads` largest of each warp's threads' maxima, on every block.
   uint32_t* maxima = reinterpret_cast<uint32_t*>(sh.pre);
   const uint32_t own_key = sort_key(own);
-  const int heads = direct ? min(32, 1 + 2 * o.k / (nb * kWarps)) : 1;
+  const int heads = direct ? min(min(32, 1024 / (nb * kWarps)), 1 + 2 * o.k / (nb * kWarps)) : 1;
   cluster.barrier_wait(std::move(started));  // every block runs: its shared memory may be written
   {
     uint32_t left = own_key;
@@ -690,7 +733,8 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     // The largest bound found by halving that at least k maxima reach; every maximum is a score,
     // so at least k scores reach it too.
     if (warp == 0) {
-      const uint32_t found = kth_bound(maxima, num_maxima, o.k, best);
+      const uint32_t found = num_maxima <= 128 ? kth_bound<4>(maxima, num_maxima, o.k)
+                                               : kth_bound<32>(maxima, num_maxima, o.k);
       if (lane == 0) sh.pick = found;
     }
     __syncthreads();
@@ -727,6 +771,35 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
 #pragma unroll
       for (int e = 0; e < C::kN; ++e) f(y[e], col + e);
     }
+  };
+  // Sum and number of the weights that `pass` lets through, gathered 32 at a time so that a warp
+  // does not evaluate a weight on every lane for the few that need it.
+  auto sum_queued = [&](auto&& pass, u64* sum, int* number) {
+    float* queue = sh.queue[warp];
+    int waiting = 0;
+    for (int c = c0; c < c1; c += 32) {
+      float y[C::kN];
+      C::unpack(c + lane < c1 ? chunk_at(c + lane) : C::masked(), y);
+      const int col = first_col(c + lane);
+#pragma unroll
+      for (int e = 0; e < C::kN; ++e) {
+        const bool in = pass(y[e], col + e);
+        const unsigned who = __ballot_sync(~0u, in);
+        if (in) queue[waiting + __popc(who & ((1u << lane) - 1))] = y[e];
+        waiting += __popc(who);
+        *number += in;
+        if (waiting >= 32) {
+          __syncwarp();
+          *sum += w(queue[lane]);
+          const float rest = queue[32 + lane];
+          __syncwarp();
+          queue[lane] = rest;
+          waiting -= 32;
+        }
+      }
+    }
+    __syncwarp();
+    if (lane < waiting) *sum += w(queue[lane]);
   };
   int turn = 0;
   auto cluster_sum = [&](u64 v) {
@@ -785,13 +858,11 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     }
   };
   auto before_warp = [&](u64* z) {
-    u64 before = 0, all = 0;
-    for (int i = 0; i < nb * kWarps; ++i) {
-      if (i == rank * kWarps + warp) before = all;
-      all += sh.tot[i];
-    }
-    *z = all;
-    return before;
+    static_assert(kMaxCluster * kWarps == 64, "two totals a lane");
+    const int me = rank * kWarps + warp, all = nb * kWarps;
+    const u64 a = lane < all ? sh.tot[lane] : 0, b = 32 + lane < all ? sh.tot[32 + lane] : 0;
+    *z = warp_reduce(a + b, Add());
+    return warp_reduce((lane < me ? a : 0) + (32 + lane < me ? b : 0), Add());
   };
   // Edge of the shortest prefix, among the columns up to `in`, whose sum of value(x) reaches
   // target: the score one 8-bit digit at a time, then the column among those that share it.
@@ -855,7 +926,7 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     const u64 in = edge;
     auto inside = [&](float y, int col) { return !limited || element(sort_key(y), col) >= in; };
     // Bins of (m - x) / T. A bin sums weights relative to its upper end, in 1 / unit, from a
-    // second-order series: good to 1e-5, which the bracket's margin covers. The edge's weight is
+    // second-order series: good to half a unit and 1e-6. The edge's weight is
     // at least (1 - p) / cols of the largest: bins beyond that are not needed.
     const float per_unit = kBinsPerUnit / t;
     const bool binned = !w.top_inf && per_unit > 0.f && per_unit < INFINITY;
@@ -863,7 +934,7 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     const float reach_units = logf(static_cast<float>(cols) / (1.f - fmaxf(o.tp, 0.f)));
     const int bins = min(kBins, static_cast<int>(reach_units * kBinsPerUnit) + 2);
     unsigned* hist = reinterpret_cast<unsigned*>(sh.wts);
-    float* hist_total = reinterpret_cast<float*>(sh.list);
+    float* hist_total = reinterpret_cast<float*>(sh.pre);
     for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
     __syncthreads();
     u64 z = 0;
@@ -882,13 +953,17 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     if (binned) {
       const int share = kBins / nb;
       for (int i = rank * share + tid; i < (rank + 1) * share; i += kThreads) {
+        unsigned part[kMaxCluster];
+#pragma unroll
+        for (int b = 0; b < kMaxCluster; ++b)
+          part[b] = b < nb ? cluster.map_shared_rank(hist, b)[i] : 0;
         float sum = 0.f;
-        for (int b = 0; b < nb; ++b)
-          sum += static_cast<float>(
-              cluster.map_shared_rank(reinterpret_cast<unsigned*>(sh.wts), b)[i]);
+#pragma unroll
+        for (int b = 0; b < kMaxCluster; ++b) sum += static_cast<float>(part[b]);
         sum *= expf(-static_cast<float>(i) / kBinsPerUnit) / unit;
-        for (int b = 0; b < nb; ++b)
-          cluster.map_shared_rank(reinterpret_cast<float*>(sh.list), b)[i] = sum;
+#pragma unroll
+        for (int b = 0; b < kMaxCluster; ++b)
+          if (b < nb) cluster.map_shared_rank(hist_total, b)[i] = sum;
       }
       if (rank == 0 && tid == 0) {
         sh.list_n = 0;
@@ -907,7 +982,7 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
       u64 run = block_scan(part, sh.red, &all);
       const double scale = exp2(static_cast<double>(-frac)) * kFix;
       const double goal = static_cast<double>(target) * scale;
-      const double margin = 4e-5 * static_cast<double>(z) * scale;
+      const double margin = (0.6 / unit + 2e-6) * static_cast<double>(z) * scale;
       for (int i = 0; i < kPer; ++i) {
         const double lo = static_cast<double>(run);
         run += static_cast<u64>(hist_total[tid * kPer + i] * kFix);
@@ -918,20 +993,16 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
       if (tid == 0 && !(goal - margin > 0.0)) sh.bracket[0] = 0;
       __syncthreads();
       const int first = static_cast<int>(sh.bracket[0]), last = static_cast<int>(sh.bracket[1]);
-      cluster.sync();  // no block looks at hist_total any more: the list may be written
       u64 sum = 0;
       int over = 0;
-      each([&](float y, int col) {
+      sum_queued([&](float y, int col) {
         const float v = (m - y) * per_unit;
-        if (!(v < static_cast<float>(last + 1)) || !inside(y, col)) return;
-        if (v < static_cast<float>(first)) {
-          sum += w(y);
-          ++over;
-        } else {
-          const unsigned at = atomicAdd(&zero->list_n, 1u);
-          if (at < kList) zero->list[at] = element(sort_key(y), static_cast<uint32_t>(col));
-        }
-      });
+        if (!(v < static_cast<float>(last + 1)) || !inside(y, col)) return false;
+        if (v < static_cast<float>(first)) return true;
+        const unsigned at = atomicAdd(&zero->list_n, 1u);
+        if (at < kList) zero->list[at] = element(sort_key(y), static_cast<uint32_t>(col));
+        return false;
+      }, &sum, &over);
       sum = warp_reduce(sum, Add());
       over = __reduce_add_sync(~0u, over);
       if (lane == 0) {
@@ -941,35 +1012,30 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
       cluster.sync();
       if (rank == 0) {
         const int n = static_cast<int>(sh.list_n);
-        u64 above = 0;
-        for (int i = 0; i < nb * kWarps; ++i) above += sh.tot[i];
-        __syncthreads();
+        u64 above;
+        before_warp(&above);
         if (tid == 0) sh.state = 0;
+        __syncthreads();
         if (n > 0 && n <= kList && above < target) {
-          const int n2 = n <= 256 ? 256 : n <= 512 ? 512 : kList, per = n2 / kThreads;
-          for (int i = n + tid; i < n2; i += kThreads) sh.list[i] = 0;
-          sort_list(sh.list, n2);
-          u64 part2 = 0, all2;
-          for (int i = tid * per; i < (tid + 1) * per; ++i) {
-            sh.wts[i] = i < n ? w(keys::order_value(element_key(sh.list[i]))) : 0;
-            part2 += sh.wts[i];
-          }
-          u64 run2 = above + block_scan(part2, sh.red, &all2);
-          for (int i = tid * per; i < (tid + 1) * per; ++i) {
-            if (run2 >= target) break;
-            const u64 v = sh.wts[i];
-            if (i < n) {  // kept, whether or not it is the last
-              const int g = static_cast<int>((element_col(sh.list[i]) + static_cast<unsigned>(head))
-                                             / C::kN);
-              atomicAdd(&sh.tot[g / block_chunks * kWarps + g % block_chunks / warp_chunks], v);
-            }
-            run2 += v;
-            if (run2 >= target) {
-              sh.edge = sh.list[i];
-              sh.state = o.mp_key > element_key(sh.list[i]) ? 1 : 2;
-              sh.cnt += i + 1;
+          for (int i = tid; i < n; i += kThreads)
+            sh.wts[i] = w(keys::order_value(element_key(sh.list[i])));
+          __syncthreads();
+          int kept = 0;
+          for (int i = tid; i < n; i += kThreads) {
+            const u64 e = sh.list[i], own = sh.wts[i];
+            u64 run = above;
+#pragma unroll 4
+            for (int j = 0; j < n; ++j) run += sh.list[j] > e ? sh.wts[j] : 0;
+            if (run >= target) continue;
+            ++kept;
+            const int g = static_cast<int>((element_col(e) + static_cast<unsigned>(head)) / C::kN);
+            atomicAdd(&sh.tot[g / block_chunks * kWarps + g % block_chunks / warp_chunks], own);
+            if (run + own >= target) {
+              sh.edge = e;
+              sh.state = o.mp_key > element_key(e) ? 1 : 2;
             }
           }
+          atomicAdd(&sh.cnt, kept);
         }
         __syncthreads();
         for (int b = 1; b < nb; ++b) {
