@@ -91,11 +91,11 @@ struct Weigher {
     m = top_inf ? 0.0 : max;
     rate = 23.083120654223414 / static_cast<double>(t);
     const double low = m - static_cast<double>(t) * 0.6931471805599453 * (frac + 1);
-    cut = top_inf ? INFINITY : fmaxf(__double2float_ru(low), -3.402823466e38f);
+    cut = fmaxf(__double2float_ru(low), -3.402823466e38f);
   }
+  // Without a branch, so that several weights are under way at once.
   __device__ __forceinline__ u64 operator()(float x) const {
-    if (!(x >= cut)) return 0;
-    if (top_inf) return u64{1} << frac;
+    if (top_inf) x = x == INFINITY ? 0.f : -INFINITY;
     const double magic = 6755399441055744.0;  // 1.5 * 2^52
     const double d = static_cast<double>(x) - m;
     const double r = fma(d, rate, magic);
@@ -109,7 +109,8 @@ struct Weigher {
     const double scaled = __hiloint2double(__double2hiint(s) + (frac + (n >> 4)) * (1 << 20),
                                            __double2loint(s));
     const double w = fma(p, scaled, 4503599627370496.0);
-    return static_cast<u64>(__double_as_longlong(w)) & ((u64{1} << 52) - 1);
+    const u64 bits = static_cast<u64>(__double_as_longlong(w)) & ((u64{1} << 52) - 1);
+    return x >= cut ? bits : 0;
   }
 };
 
@@ -174,7 +175,6 @@ struct Shared {
   u64 xch[2][kMaxCluster];        // cluster_sum
   u64 red[kWarps];
   double table[16];
-  float queue[kWarps][64];
   u64 edge;            // what block 0 found out
   u64 above;
   int state;
@@ -755,8 +755,11 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     cluster.sync();
     const unsigned n = zero->list_n;
     if (n <= kList) {
-      if (nb > 1) cluster.sync();  // block 0's count has been read
-      if (rank == 0) finish_list(p, row, static_cast<int>(n), o, w, sh);
+      // block 0 stays until the others have read its count
+      auto read = cluster.barrier_arrive();
+      if (rank != 0) return;
+      finish_list(p, row, static_cast<int>(n), o, w, sh);
+      cluster.barrier_wait(std::move(read));
       return;
     }
   }
@@ -772,34 +775,33 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
       for (int e = 0; e < C::kN; ++e) f(y[e], col + e);
     }
   };
-  // Sum and number of the weights that `pass` lets through, gathered 32 at a time so that a warp
-  // does not evaluate a weight on every lane for the few that need it.
-  auto sum_queued = [&](auto&& pass, u64* sum, int* number) {
-    float* queue = sh.queue[warp];
-    int waiting = 0;
-    for (int c = c0; c < c1; c += 32) {
-      float y[C::kN];
-      C::unpack(c + lane < c1 ? chunk_at(c + lane) : C::masked(), y);
-      const int col = first_col(c + lane);
+  // Sum and number of the weights that `pass` lets through. Each lane marks those among 32 of its
+  // scores first and then weighs its marked ones, so that a warp does not weigh every score for
+  // the few that need it.
+  auto sum_chosen = [&](auto&& pass, u64* sum, int* number) {
+    constexpr int kGroup = 32 / C::kN;
+    for (int c = c0 + lane; c < c1; c += 32 * kGroup) {
+      uint32_t marked = 0;
 #pragma unroll
-      for (int e = 0; e < C::kN; ++e) {
-        const bool in = pass(y[e], col + e);
-        const unsigned who = __ballot_sync(~0u, in);
-        if (in) queue[waiting + __popc(who & ((1u << lane) - 1))] = y[e];
-        waiting += __popc(who);
-        *number += in;
-        if (waiting >= 32) {
-          __syncwarp();
-          *sum += w(queue[lane]);
-          const float rest = queue[32 + lane];
-          __syncwarp();
-          queue[lane] = rest;
-          waiting -= 32;
-        }
+      for (int i = 0; i < kGroup; ++i) {
+        const int at = c + i * 32;
+        if (at >= c1) break;
+        float y[C::kN];
+        C::unpack(chunk_at(at), y);
+        const int col = first_col(at);
+#pragma unroll
+        for (int e = 0; e < C::kN; ++e)
+          marked |= pass(y[e], col + e) ? 1u << (i * C::kN + e) : 0u;
+      }
+      *number += __popc(marked);
+      while (marked) {
+        const int bit = __ffs(marked) - 1;
+        marked &= marked - 1;
+        const int at = c + bit / C::kN * 32, e = bit % C::kN;
+        *sum += w(score_f32(at < resident ? reinterpret_cast<const T*>(held + at)[e]
+                                          : x[first_col(at) + e]));
       }
     }
-    __syncwarp();
-    if (lane < waiting) *sum += w(queue[lane]);
   };
   int turn = 0;
   auto cluster_sum = [&](u64 v) {
@@ -937,17 +939,22 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     float* hist_total = reinterpret_cast<float*>(sh.pre);
     for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
     __syncthreads();
+    const float bins_f = binned ? static_cast<float>(bins) : 0.f;
     u64 z = 0;
-    each([&](float y, int col) {
-      if (!inside(y, col)) return;
-      z += w(y);
-      if (!binned) return;
-      const float v = (m - y) * per_unit;
-      if (!(v < static_cast<float>(bins))) return;
-      const int b = static_cast<int>(v);
-      const float f = (v - static_cast<float>(b)) * (1.f / kBinsPerUnit);
-      atomicAdd(&hist[b], static_cast<unsigned>(__float2int_rn(unit * (1.f - f * (1.f - 0.5f * f)))));
-    });
+    auto weigh = [&](float y, bool in) {
+      const u64 own = w(y);
+      z += in ? own : 0;
+      // the nearest bin below, and how far into it, without a conversion
+      const float v = (m - y) * per_unit, vb = __fadd_rz(v, 8388608.f);
+      const float f = (v - (vb - 8388608.f)) * (1.f / kBinsPerUnit);
+      const float q = fmaf(unit, 1.f - f * (1.f - 0.5f * f), 8388608.f);
+      if (v < bins_f && in)
+        atomicAdd(&hist[__float_as_uint(vb) & 0x7fffffu], __float_as_uint(q) - 0x4b000000u);
+    };
+    if (limited)
+      each([&](float y, int col) { weigh(y, element(sort_key(y), col) >= in); });
+    else
+      each([&](float y, int) { weigh(y, true); });
     z = cluster_sum(z);
     const u64 target = top_p_target(o.tp, z);
     if (binned) {
@@ -993,12 +1000,15 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
       if (tid == 0 && !(goal - margin > 0.0)) sh.bracket[0] = 0;
       __syncthreads();
       const int first = static_cast<int>(sh.bracket[0]), last = static_cast<int>(sh.bracket[1]);
+      // the bracket in scores, a little wider than the bins
+      const float slack = 4e-7f * (fabsf(m) + static_cast<float>(last + 1) / per_unit);
+      const float high = m - static_cast<float>(first) / per_unit + slack;
+      const float low = m - static_cast<float>(last + 1) / per_unit - slack;
       u64 sum = 0;
       int over = 0;
-      sum_queued([&](float y, int col) {
-        const float v = (m - y) * per_unit;
-        if (!(v < static_cast<float>(last + 1)) || !inside(y, col)) return false;
-        if (v < static_cast<float>(first)) return true;
+      sum_chosen([&](float y, int col) {
+        if (!(y >= low) || !inside(y, col)) return false;
+        if (y >= high) return true;
         const unsigned at = atomicAdd(&zero->list_n, 1u);
         if (at < kList) zero->list[at] = element(sort_key(y), static_cast<uint32_t>(col));
         return false;
