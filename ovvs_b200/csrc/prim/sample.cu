@@ -48,6 +48,7 @@ constexpr int kRankList = 256;  // up to here it counts instead of sorting
 constexpr int kDirectK = 448;   // the largest top_k that the list serves
 constexpr int kRound = 8;       // chunks a thread has in flight where one block takes the row
 constexpr int kWanted = 520;    // columns it means to list
+constexpr int kNoted = 16;      // chunks a thread can note there
 constexpr int kBins = 2048;
 constexpr float kBinsPerUnit = 64.f;  // histogram bins per unit of (m - x) / T
 static_assert(kBins * sizeof(float) == kList * sizeof(uint64_t), "the list holds the histogram");
@@ -185,6 +186,8 @@ struct Shared {
   int found;
   int cnt;
 };
+static_assert(sizeof(int) * kNoted * kThreads == 2 * sizeof(u64) * kList,
+              "wts and pre hold the noted chunks");
 static_assert(sizeof(uint32_t) * kMaxCluster * kThreads == sizeof(u64) * kList, "maxima fit");
 
 template <class V, class Op>
@@ -497,8 +500,12 @@ __device__ void finish_list(const SampleParams& p, int64_t row, int n, const Set
   }
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads, 4)
+// kBlocks: blocks an SM is meant to hold. Where one block takes a row, five of 48 registers a
+// thread stream better than four of 64 (1000 rows of 100,000 fp32: 113 us against 134); where a
+// cluster does, the weights want the registers (256 rows of 100,003 fp16, top-p: 183 us against
+// 197).
+template <class T, int kBlocks>
+__global__ void __launch_bounds__(kThreads, kBlocks)
 sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
   using C = Chunk<T>;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -604,45 +611,36 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     }
     __syncthreads();
     const float bound = keys::order_value(sh.pick);
+    // Each thread notes its chunks that reach the bound (some kWanted of all threads' together)
+    // and lists their columns afterwards: the pass itself has no atomic and no vote.
+    int* noted = reinterpret_cast<int*>(sh.wts) + tid;
+    int count = 0;
     for (int r = 0; r < rounds; ++r) {
       load_round(r);
-      unsigned count = 0;
 #pragma unroll
       for (int i = 0; i < kRound; ++i) {
-        if (!(C::largest(v[i]) >= bound)) continue;
-        float y[C::kN];
-        C::unpack(v[i], y);
-#pragma unroll
-        for (int e = 0; e < C::kN; ++e) count += y[e] >= bound;
-      }
-      if (!__ballot_sync(~0u, count)) continue;
-      unsigned at = count;  // places for the whole warp at once
-#pragma unroll
-      for (int i = 1; i < 32; i <<= 1) {
-        const unsigned y = __shfl_up_sync(~0u, at, i);
-        if (lane >= i) at += y;
-      }
-      unsigned base_at = 0;
-      if (lane == 31) base_at = atomicAdd(&sh.list_n, at);
-      at += __shfl_sync(~0u, base_at, 31) - count;
-      if (count == 0) continue;
-#pragma unroll
-      for (int i = 0; i < kRound; ++i) {
-        if (!(C::largest(v[i]) >= bound)) continue;
-        float y[C::kN];
-        C::unpack(v[i], y);
-        const int col = first_col((r * kRound + i) * kThreads + tid);
-#pragma unroll
-        for (int e = 0; e < C::kN; ++e) {
-          if (!(y[e] >= bound)) continue;
-          if (at < kList) sh.list[at] = element(sort_key(y[e]), static_cast<uint32_t>(col + e));
-          ++at;
+        if (C::largest(v[i]) >= bound) {
+          if (count < kNoted) noted[count * kThreads] = (r * kRound + i) * kThreads + tid;
+          ++count;
         }
+      }
+    }
+    const bool fits = !__syncthreads_or(count > kNoted);
+    for (int i = 0; i < count && fits; ++i) {
+      const int c = noted[i * kThreads];
+      float y[C::kN];
+      C::unpack(fetch(c), y);
+#pragma unroll
+      for (int e = 0; e < C::kN; ++e) {
+        if (!(y[e] >= bound)) continue;
+        const unsigned at = atomicAdd(&sh.list_n, 1u);
+        if (at < kList)
+          sh.list[at] = element(sort_key(y[e]), static_cast<uint32_t>(first_col(c) + e));
       }
     }
     __syncthreads();
     unsigned listed = sh.list_n;
-    if (listed <= kList) {
+    if (fits && listed <= kList) {
       if (listed > static_cast<unsigned>(o.k + o.k / 4)) {
         const uint32_t lo = list_bound(sh, static_cast<int>(listed), o.k, sh.pick);
         listed = keep_listed(sh, static_cast<int>(listed), lo);
@@ -1111,20 +1109,22 @@ cudaError_t sample(const SampleParams& p, cudaStream_t stream) {
   constexpr int kN = Chunk<T>::kN;
   constexpr size_t kFixed = (sizeof(Shared) + 15) / 16 * 16;
   const int64_t chunks = (p.cols + 2 * kN - 2) / kN;  // whatever the row's alignment
-  int nb = 1;
+  // A batch that fills the GPU with one block a row, and may have top-k rows, which that block
+  // then reads in one pass; otherwise up to a cluster a row, of blocks of 512 chunks or more.
   const bool one_pass = p.top_k && p.rows >= 296;
+  int nb = 1;
   while (nb < kMaxCluster && chunks / nb > 512 && !one_pass) nb *= 2;
   const int block_chunks = static_cast<int>((chunks + nb - 1) / nb);
-  const int most = static_cast<int>(((one_pass ? 56 : 227) * 1024 - kFixed) / 16);
+  const int most = static_cast<int>(((one_pass ? 45 : 227) * 1024 - kFixed) / 16);
   const int resident = block_chunks < most ? block_chunks : most;
-  const size_t smem = kFixed + static_cast<size_t>(resident) * 16;
-  cudaError_t e = cudaFuncSetAttribute(
-      sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  auto kernel = one_pass ? sample_kernel<T, 5> : sample_kernel<T, 4>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       227 * 1024);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(p.rows * nb));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = kFixed + static_cast<size_t>(resident) * 16;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -1132,7 +1132,7 @@ cudaError_t sample(const SampleParams& p, cudaStream_t stream) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_kernel<T>, p, frac_bits(p.cols), block_chunks, resident);
+  return cudaLaunchKernelEx(&cfg, kernel, p, frac_bits(p.cols), block_chunks, resident);
 }
 
 }  // namespace
