@@ -49,8 +49,7 @@ constexpr int kDirectK = 448;   // the largest top_k that the list serves
 constexpr int kRound = 8;       // chunks a thread has in flight where one block takes the row
 constexpr int kWanted = 520;    // columns it means to list
 constexpr int kNoted = 16;      // chunks a thread can note there
-constexpr int kBins = 2048;
-constexpr float kBinsPerUnit = 64.f;  // histogram bins per unit of (m - x) / T
+constexpr int kBins = 2048;     // of the weight histogram
 static_assert(kBins * sizeof(float) == kList * sizeof(uint64_t), "the list holds the histogram");
 
 using u64 = unsigned long long;
@@ -169,9 +168,10 @@ __device__ __forceinline__ void Chunk<__nv_bfloat16>::unpack(const uint4& v, flo
 }
 
 struct Shared {
-  u64 list[kList];     // candidates; the histogram's totals before there are any
+  u64 list[kList];     // candidates (block 0)
   u64 wts[kList];      // their weights; the histogram before there are any
-  u64 pre[kList];      // running sums; the threads' maxima before there are any
+  u64 pre[kList];      // running sums; before them maxima, the histogram's totals, columns on
+                       // their way to block 0
   u64 tot[kMaxCluster * kWarps];  // kept weight of every warp of the cluster
   u64 xch[2][kMaxCluster];        // cluster_sum
   u64 red[kWarps];
@@ -180,6 +180,7 @@ struct Shared {
   u64 above;
   int state;
   unsigned list_n;
+  unsigned staged;
   unsigned pick;
   unsigned bracket[2];
   unsigned first;
@@ -576,6 +577,7 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
   if (tid < 16) sh.table[tid] = kSixteenths[tid];
   if (tid == 0) {
     sh.list_n = 0;
+    sh.staged = 0;
     sh.first = ~0u;
   }
   auto started = cluster.barrier_arrive();
@@ -699,6 +701,19 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
   }
   const float m = keys::order_value(best);
   Shared* zero = cluster.map_shared_rank(&sh, 0);
+  // Columns for block 0's list wait in this block's `pre` and go over together.
+  auto stage = [&](float y, int col) {
+    const unsigned at = atomicAdd(&sh.staged, 1u);
+    if (at < kList) sh.pre[at] = element(sort_key(y), static_cast<uint32_t>(col));
+  };
+  auto hand_over = [&] {
+    __syncthreads();
+    const unsigned n = sh.staged;
+    if (tid == 0 && n) sh.pick = atomicAdd(&zero->list_n, n);
+    __syncthreads();
+    for (unsigned i = tid; i < n && i < kList; i += kThreads)
+      if (sh.pick + i < kList) zero->list[sh.pick + i] = sh.pre[i];
+  };
 
   if (greedy) {  // the first column that holds the largest score
     unsigned first = ~0u;
@@ -745,11 +760,10 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
       C::unpack(v, y);
 #pragma unroll
       for (int e = 0; e < C::kN; ++e) {
-        if (!(y[e] >= bound)) continue;
-        const unsigned at = atomicAdd(&zero->list_n, 1u);
-        if (at < kList) zero->list[at] = element(sort_key(y[e]), first_col(c) + e);
+        if (y[e] >= bound) stage(y[e], first_col(c) + e);
       }
     }
+    hand_over();
     cluster.sync();
     const unsigned n = zero->list_n;
     if (n <= kList) {
@@ -773,32 +787,34 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
       for (int e = 0; e < C::kN; ++e) f(y[e], col + e);
     }
   };
-  // Sum and number of the weights that `pass` lets through. Each lane marks those among 32 of its
-  // scores first and then weighs its marked ones, so that a warp does not weigh every score for
-  // the few that need it.
-  auto sum_chosen = [&](auto&& pass, u64* sum, int* number) {
+  // f(score, column) for the scores from `high` on, g for those below it from `low` on. Each lane
+  // marks them among 32 of its scores first and then takes its marked ones, so that a warp does
+  // not go through the motions of f on every score for the few that need it.
+  auto each_from = [&](float low, float high, auto&& f, auto&& g) {
     constexpr int kGroup = 32 / C::kN;
+    low = fmaxf(low, -3.402823466e38f);  // -inf stands where there is no column
+    high = fmaxf(high, low);
     for (int c = c0 + lane; c < c1; c += 32 * kGroup) {
-      uint32_t marked = 0;
+      uint32_t above = 0, within = 0;
 #pragma unroll
       for (int i = 0; i < kGroup; ++i) {
-        const int at = c + i * 32;
-        if (at >= c1) break;
         float y[C::kN];
-        C::unpack(chunk_at(at), y);
-        const int col = first_col(at);
+        C::unpack(c + i * 32 < c1 ? chunk_at(c + i * 32) : C::masked(), y);
 #pragma unroll
-        for (int e = 0; e < C::kN; ++e)
-          marked |= pass(y[e], col + e) ? 1u << (i * C::kN + e) : 0u;
+        for (int e = 0; e < C::kN; ++e) {
+          above |= y[e] >= high ? 1u << (i * C::kN + e) : 0u;
+          within |= y[e] >= low ? 1u << (i * C::kN + e) : 0u;
+        }
       }
-      *number += __popc(marked);
-      while (marked) {
-        const int bit = __ffs(marked) - 1;
-        marked &= marked - 1;
-        const int at = c + bit / C::kN * 32, e = bit % C::kN;
-        *sum += w(score_f32(at < resident ? reinterpret_cast<const T*>(held + at)[e]
-                                          : x[first_col(at) + e]));
-      }
+      within &= ~above;
+      auto take = [&](uint32_t& bits, auto&& h) {
+        const int bit = __ffs(bits) - 1;
+        bits &= bits - 1;
+        const int at = c + bit / C::kN * 32, e = bit % C::kN, col = first_col(at) + e;
+        h(score_f32(at < resident ? reinterpret_cast<const T*>(held + at)[e] : x[col]), col);
+      };
+      while (within) take(within, g);
+      while (above) take(above, f);
     }
   };
   int turn = 0;
@@ -811,10 +827,8 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     for (int b = 0; b < nb; ++b) s += sh.xch[turn][b];
     return s;
   };
-  // Sum of value(x, col) of every warp, on every block.
-  auto warp_totals = [&](auto&& value) {
-    u64 s = 0;
-    each([&](float y, int col) { s += value(y, col); });
+  // Sum over the lanes of every warp, on every block.
+  auto share_totals = [&](u64 s) {
     s = warp_reduce(s, Add());
     cluster.sync();
     if (lane < nb) cluster.map_shared_rank(&sh, lane)->tot[rank * kWarps + warp] = s;
@@ -900,8 +914,9 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
       const uint32_t k = sort_key(y);
       return u64{k == prefix && element(k, col) >= in};
     };
-    warp_totals(tie);
-    u64 all;
+    u64 own_ties = 0, all;
+    each([&](float y, int col) { own_ties += tie(y, col); });
+    share_totals(own_ties);
     const u64 before = before_warp(&all);
     if (ties - 1 >= before && ties - 1 < before + sh.tot[rank * kWarps + warp])
       walk(before, ties - 1, tie, [&](int col, u64) {
@@ -925,26 +940,27 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     const bool limited = edge != everything;
     const u64 in = edge;
     auto inside = [&](float y, int col) { return !limited || element(sort_key(y), col) >= in; };
-    // Bins of (m - x) / T. A bin sums weights relative to its upper end, in 1 / unit, from a
-    // second-order series: good to half a unit and 1e-6. The edge's weight is
-    // at least (1 - p) / cols of the largest: bins beyond that are not needed.
-    const float per_unit = kBinsPerUnit / t;
+    // Bins of (m - x) / T. The edge's weight is at least (1 - p) / cols of the largest, so they
+    // reach that far and no further: 100 to 200 a unit. A bin sums weights relative to its upper
+    // end, in 1 / unit, from a second-order series: good to half a unit and 1e-6.
+    const float reach_units = logf(static_cast<float>(cols) / (1.f - fmaxf(o.tp, 0.f))) + 0.1f;
+    const float bins_per_unit = kBins / reach_units;
+    const float per_unit = bins_per_unit / t;
     const bool binned = !w.top_inf && per_unit > 0.f && per_unit < INFINITY;
     const float unit = fminf(65536.f, 4294967040.f / (static_cast<float>(block_chunks) * C::kN));
-    const float reach_units = logf(static_cast<float>(cols) / (1.f - fmaxf(o.tp, 0.f)));
-    const int bins = min(kBins, static_cast<int>(reach_units * kBinsPerUnit) + 2);
     unsigned* hist = reinterpret_cast<unsigned*>(sh.wts);
     float* hist_total = reinterpret_cast<float*>(sh.pre);
     for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
     __syncthreads();
-    const float bins_f = binned ? static_cast<float>(bins) : 0.f;
+    const float bins_f = binned ? static_cast<float>(kBins) : 0.f;
+    const float unit_per_bin = 1.f / bins_per_unit;
     u64 z = 0;
     auto weigh = [&](float y, bool in) {
       const u64 own = w(y);
       z += in ? own : 0;
       // the nearest bin below, and how far into it, without a conversion
       const float v = (m - y) * per_unit, vb = __fadd_rz(v, 8388608.f);
-      const float f = (v - (vb - 8388608.f)) * (1.f / kBinsPerUnit);
+      const float f = (v - (vb - 8388608.f)) * unit_per_bin;
       const float q = fmaf(unit, 1.f - f * (1.f - 0.5f * f), 8388608.f);
       if (v < bins_f && in)
         atomicAdd(&hist[__float_as_uint(vb) & 0x7fffffu], __float_as_uint(q) - 0x4b000000u);
@@ -965,7 +981,7 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
         float sum = 0.f;
 #pragma unroll
         for (int b = 0; b < kMaxCluster; ++b) sum += static_cast<float>(part[b]);
-        sum *= expf(-static_cast<float>(i) / kBinsPerUnit) / unit;
+        sum *= expf(-static_cast<float>(i) * unit_per_bin) / unit;
 #pragma unroll
         for (int b = 0; b < kMaxCluster; ++b)
           if (b < nb) cluster.map_shared_rank(hist_total, b)[i] = sum;
@@ -975,7 +991,8 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
         sh.cnt = 0;
       }
       if (tid == 0) {
-        sh.bracket[0] = sh.bracket[1] = static_cast<unsigned>(bins - 1);
+        sh.staged = 0;
+        sh.bracket[0] = sh.bracket[1] = kBins - 1;
       }
       cluster.sync();
       // the bins where the running sum surely has not, and surely has, reached the target
@@ -1004,13 +1021,16 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
       const float low = m - static_cast<float>(last + 1) / per_unit - slack;
       u64 sum = 0;
       int over = 0;
-      sum_chosen([&](float y, int col) {
-        if (!(y >= low) || !inside(y, col)) return false;
-        if (y >= high) return true;
-        const unsigned at = atomicAdd(&zero->list_n, 1u);
-        if (at < kList) zero->list[at] = element(sort_key(y), static_cast<uint32_t>(col));
-        return false;
-      }, &sum, &over);
+      each_from(low, high,
+                [&](float y, int col) {
+                  if (!inside(y, col)) return;
+                  sum += w(y);
+                  ++over;
+                },
+                [&](float y, int col) {
+                  if (inside(y, col)) stage(y, col);
+                });
+      hand_over();
       sum = warp_reduce(sum, Add());
       over = __reduce_add_sync(~0u, over);
       if (lane == 0) {
@@ -1028,13 +1048,18 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
           for (int i = tid; i < n; i += kThreads)
             sh.wts[i] = w(keys::order_value(element_key(sh.list[i])));
           __syncthreads();
+          const int share = n <= 32 ? 8 : n <= 64 ? 4 : n <= 128 ? 2 : 1;
           int kept = 0;
-          for (int i = tid; i < n; i += kThreads) {
-            const u64 e = sh.list[i], own = sh.wts[i];
-            u64 run = above;
+          for (int i0 = 0; i0 < n; i0 += kThreads / share) {
+            const int i = i0 + tid / share;
+            const u64 e = i < n ? sh.list[i] : ~u64{0};
+            u64 run = 0;
 #pragma unroll 4
-            for (int j = 0; j < n; ++j) run += sh.list[j] > e ? sh.wts[j] : 0;
-            if (run >= target) continue;
+            for (int j = tid % share; j < n; j += share) run += sh.list[j] > e ? sh.wts[j] : 0;
+            for (int s = 1; s < share; s <<= 1) run += __shfl_xor_sync(~0u, run, s);
+            run += above;
+            if (i >= n || tid % share || run >= target) continue;
+            const u64 own = sh.wts[i];
             ++kept;
             const int g = static_cast<int>((element_col(e) + static_cast<unsigned>(head)) / C::kN);
             atomicAdd(&sh.tot[g / block_chunks * kWarps + g % block_chunks / warp_chunks], own);
@@ -1066,12 +1091,23 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     return element(sort_key(y), col) >= edge ? w(y) : u64{0};
   };
   if (!summed) {
-    u64 n = 0;
-    warp_totals([&](float y, int col) {
-      const bool keep = element(sort_key(y), col) >= edge;
-      n += keep;
-      return keep ? w(y) : u64{0};
-    });
+    u64 sum = 0, n = 0;
+    if (edge == everything) {
+      each([&](float y, int) {
+        sum += w(y);
+        n += y > -INFINITY;
+      });
+    } else {
+      auto take = [&](float y, int) {
+        sum += w(y);
+        ++n;
+      };
+      const float last = keys::order_value(element_key(edge));
+      each_from(last, keys::order_value(element_key(edge) + 1), take, [&](float y, int col) {
+        if (static_cast<uint32_t>(col) <= element_col(edge)) take(y, col);
+      });
+    }
+    share_totals(sum);
     if (p.kept) {
       n = cluster_sum(n);
       if (rank == 0 && tid == 0) p.kept[row] = static_cast<int>(n);
