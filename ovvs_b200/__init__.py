@@ -183,8 +183,15 @@ def _dev_ptr(t) -> c_void_p:
     return c_void_p(int(t))
 
 
+_type_names: dict = {}
+
+
 def _type_name(t) -> str:
-    return str(t.dtype).rsplit(".", 1)[-1]
+    """"float32" for an array of torch.float32; the names are kept by dtype."""
+    name = _type_names.get(t.dtype)
+    if name is None:
+        name = _type_names[t.dtype] = str(t.dtype).rsplit(".", 1)[-1]
+    return name
 
 
 class Resources:
@@ -350,7 +357,7 @@ class Resources:
         return nb, ds
 
     # Rows of scores on the GPU (include/ovvs/ovvs_cuda.h). The arguments are CUDA tensors
-    # (objects with data_ptr(), shape, stride(), dtype and device, e.g. torch's); outputs are
+    # (torch's, or objects with the methods of theirs that are used below); outputs are
     # written in place. Work is enqueued on `stream` (a cudaStream_t as an integer; None: this
     # Resources' own stream, 0: the default stream) and not waited for.
     def _device_scores(self, t, what):
@@ -369,22 +376,23 @@ class Resources:
         return self._on_device(t, what), type_, rows, cols, stride[0] if rows > 1 else cols
 
     def _on_device(self, t, what):
-        if self._device is None:
+        if t.get_device() != self._device:
             self._device = self.device()
-        d = t.device
-        if d.type != "cuda" or d.index != self._device:
-            raise ValueError(f"{what} is on {d}, not on cuda:{self._device}")
+            if t.get_device() != self._device:
+                raise ValueError(f"{what} is on {t.device}, not on cuda:{self._device}")
         return t.data_ptr()
 
     def _device_array(self, t, what, type_, shape):
         """Pointer of a contiguous tensor of the given type and shape (None: null)."""
         if t is None:
             return None
-        if _type_name(t) != type_:
+        if _type_names.get(t.dtype) != type_ and _type_name(t) != type_:
             raise ValueError(f"{what} must be {type_}, not {t.dtype}")
-        if tuple(t.shape) != shape or not t.is_contiguous():
+        if t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{what} must be contiguous {shape}, not {tuple(t.shape)}")
-        return self._on_device(t, what)
+        if t.get_device() != self._device:
+            self._on_device(t, what)
+        return t.data_ptr()
 
     def _stream_of(self, stream):
         return self.stream() if stream is None else int(stream)

@@ -10,11 +10,26 @@
 // share nothing.
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <cuda_runtime.h>
 
 namespace ovvs {
 namespace prim {
+
+// Opts a kernel in to `bytes` of dynamic shared memory on the current device, once per device:
+// the attribute lasts, and setting it costs more than a launch.
+template <class Kernel>
+inline cudaError_t allow_smem(Kernel* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = device < 64 ? uint64_t{1} << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
 
 // ovvsScoreType (ovvs_cuda.h).
 enum ScoreType : int { kScoreF32 = 0, kScoreF16 = 1, kScoreBf16 = 16 };

@@ -1154,8 +1154,8 @@ cudaError_t sample(const SampleParams& p, cudaStream_t stream) {
   const int most = static_cast<int>(((one_pass ? 45 : 227) * 1024 - kFixed) / 16);
   const int resident = block_chunks < most ? block_chunks : most;
   auto kernel = one_pass ? sample_kernel<T, 5> : sample_kernel<T, 4>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       227 * 1024);
+  static std::atomic<uint64_t> done[2];
+  const cudaError_t e = allow_smem(kernel, 227 * 1024, done[one_pass]);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(p.rows * nb));

@@ -104,7 +104,6 @@ def test_binding_refuses_host_tensors_and_wrong_shapes(ovvs):
     import torch
 
     res = ovvs.Resources()
-    res._device = 0
     x = torch.zeros(4, 8)
     u = torch.zeros(4)
     with pytest.raises(ValueError, match="is on cpu"):
