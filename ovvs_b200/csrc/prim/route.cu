@@ -7,10 +7,10 @@
 // chosen s).
 //
 // Which expert is chosen is what 64 bits say: two experts of one token may stand nearer than 32
-// bits tell apart. The fast way computes in 32 bits and knows how far it may be off (kDoubt): it
-// decides alone where neighbours in the order stand further apart than that, orders the few
-// doubtful experts by their 64-bit values where not, and hands a token whose groups are in doubt
-// to the plain 64-bit way.
+// bits tell apart. The fast way computes in 32 bits and knows how far it may be off: it decides
+// alone where neighbours in the order stand further apart than that, orders the few doubtful
+// experts by their 64-bit values where not, and hands a token whose groups are in doubt to the
+// plain 64-bit way.
 #include "rows.cuh"
 
 #include "keys.cuh"
@@ -23,15 +23,21 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 
-// How near two choices s + bias computed in 32 bits may stand before their order is in doubt,
-// relative to the larger of 1 and their size, in units of 2^-24. A sigmoid is off by at most 4.3:
-// the exponential's own 4, which s (1 - s) quarters, its rounded argument 1.2 |x| s (1 - s) < 0.3,
-// one rounding of the denominator, two of the reciprocal. A softmax by at most 49: the same for
-// its numerator, and its sum of up to 1024 terms. Adding the bias rounds half a unit. Both sides
-// of a pair, and twice that to be safe; sums of two choices count twice again.
-constexpr float kUnit = 5.9604645e-8f;
-constexpr float kDoubtSigmoid = 24.f * kUnit;
-constexpr float kDoubtSoftmax = 200.f * kUnit;
+// In the fast way an expert's place in the order is one 32-bit integer, its value's code above
+// and its id (lower ones larger) below, so that no two are equal and the best is one maximum;
+// 0 cannot be chosen. A value's code is
+// - without a bias the leading bits of the logit's order-preserving image: all of a 16-bit
+//   type's, so that nothing is in doubt; fp32 logits with the same leading bits are;
+// - with one, s + bias in units of 2^-20 (2^-19 for more than 256 experts) between -4 and 4; what
+//   lies beyond counts as the end of the range, and is in doubt among itself.
+// A sigmoid is off by at most 4.3 * 2^-24: the exponential's own 4, which s (1 - s) quarters, its
+// rounded argument 1.2 |x| s (1 - s) < 0.3, one rounding of the denominator, two of the
+// reciprocal. A softmax by at most 49 * 2^-24: the same for its numerator, and its sum of up to
+// 1024 terms. Adding the bias rounds by up to 4 * 2^-24 and the code by half a unit: 1.1 units
+// for a sigmoid, 3.9 for a softmax (0.6 and 2 of the coarser units, and one that is cut off).
+// Codes of a pair no further apart than twice that, rounded up, are in doubt; of sums of two,
+// twice as far and two more.
+constexpr int kNearSigmoid = 3, kNearSoftmax = 9;
 
 __device__ __forceinline__ bool better(double a, int i, double b, int j) {
   return a > b || (a == b && i < j);
@@ -76,10 +82,12 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
 // -inf and NaN are masked.
 __device__ __forceinline__ float masked(float v) { return v > -INFINITY ? v : -INFINITY; }
 
-// Position in the order as an integer: larger is earlier, 0 cannot be chosen.
-__device__ __forceinline__ uint32_t choice_key(float c) {
-  return c > -INFINITY ? keys::order_bits(c) : 0u;
+// c in units of 2^-20 above -4: c + 12 lies in [8, 16), where a float's last bit is one unit.
+// Never 0, which marks what cannot be chosen.
+__device__ __forceinline__ uint32_t fixed_code(float c) {
+  return __float_as_uint(fminf(fmaxf(c + 12.f, 8.000001f), 15.999999f)) & 0x7fffffu;
 }
+constexpr uint32_t kFixedZero = 4u << 20;  // fixed_code(0)
 
 __device__ __forceinline__ float exp_fast(float x) {  // 2^-22 and the argument's rounding
   float y;
@@ -260,13 +268,16 @@ __device__ __forceinline__ void store_cells(T* row, int e0, int n, bool whole,
 
 // The fast way: kLanes lanes take a token, each kPer neighbouring experts in registers. Groups,
 // where there are any, are whole lanes: group_lanes (a power of two) each.
-template <class T, int kLanes, int kPer>
+template <class T, int kLanes, int kPer, bool kBias>
 __global__ void __launch_bounds__(kThreads)
 route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
   extern __shared__ double smem[];
   __shared__ int ids_of[kWarps][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kIdBits = kLanes * kPer <= 256 ? 8 : 10;
+  constexpr uint32_t kIds = (1u << kIdBits) - 1;
+  constexpr int kDrop = kIdBits == 8 ? 0 : 1;  // of a code's 23 bits
   constexpr int kTokens = 32 / kLanes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane % kLanes, n = p.experts, k = p.k;
   const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * kWarps + warp) * kTokens;
   if (t0 >= p.tokens) return;
@@ -278,180 +289,190 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
 
   float v[kPer];
   load_cells<T, kPer>(x, e0, n, whole, v, -INFINITY);
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) v[i] = masked(v[i]);
-  const bool need_scores = p.bias || p.scores || (p.groups > 1 && p.group_top2);
+  const bool sums = p.groups > 1 && p.group_top2;
+  const bool need_scores = kBias || p.scores;
   float m = 0.f, inv_z = 0.f;
-  if (!p.sigmoid && (need_scores || !p.renormalize)) {
-    m = v[0];
+  if (!p.sigmoid && (need_scores || sums || !p.renormalize)) {
+    m = v[0];  // a NaN is not the larger one
 #pragma unroll
     for (int i = 1; i < kPer; ++i) m = fmaxf(m, v[i]);
-    m = lanes_max<kLanes>(m);
+    m = lanes_max<kLanes>(fmaxf(m, -INFINITY));
     float z = 0.f;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      z += v[i] > -INFINITY ? (v[i] == m ? 1.f : exp_fast(v[i] - m)) : 0.f;
+    for (int i = 0; i < kPer; ++i) {
+      const float e = v[i] == m ? 1.f : exp_fast(v[i] - m);
+      z += v[i] > -INFINITY ? e : 0.f;
+    }
     z = lanes_sum<kLanes>(z);
     inv_z = z > 0.f ? 1.f / z : 0.f;
   }
   auto score = [&](float y) {
-    if (!(y > -INFINITY)) return 0.f;
-    if (p.sigmoid) return sigmoid_fast(y);
-    return (y == m ? 1.f : exp_fast(y - m)) * inv_z;
+    const float s = p.sigmoid ? sigmoid_fast(y) : (y == m ? 1.f : exp_fast(y - m)) * inv_z;
+    return y > -INFINITY ? s : 0.f;
   };
   uint32_t key[kPer];
   if (need_scores) {
-    float s[kPer], b[kPer];
+    float s[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) s[i] = score(v[i]);
-    if (p.scores && live)
-      store_cells<float, kPer>(p.scores + t * n, e0, n, whole_scores, s);
-    if (p.bias) {
+    if (p.scores && live) store_cells<float, kPer>(p.scores + t * n, e0, n, whole_scores, s);
+    if constexpr (kBias) {
+      float b[kPer];
+      load_cells<float, kPer>(p.bias, e0, n, whole_scores, b, 0.f);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) b[i] = e0 + i < n ? __ldg(p.bias + e0 + i) : 0.f;
+      for (int i = 0; i < kPer; ++i) {
+        const float c = s[i] + b[i];
+        const bool can = v[i] > -INFINITY && c > -INFINITY;
+        key[i] = can ? fixed_code(c) >> kDrop << kIdBits | (kIds - (e0 + i)) : 0u;
+      }
     }
+  }
+  if constexpr (!kBias) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      key[i] = v[i] > -INFINITY ? choice_key(p.bias ? s[i] + b[i] : v[i]) : 0u;
-  } else {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) key[i] = choice_key(v[i]);
+      key[i] = v[i] > -INFINITY ? (keys::order_bits(v[i]) & ~kIds) | (kIds - (e0 + i)) : 0u;
   }
-  const float doubt = p.sigmoid ? kDoubtSigmoid : kDoubtSoftmax;
-  auto near = [&](float a, float b) {
-    return a - b <= doubt * fmaxf(1.f, fmaxf(fabsf(a), fabsf(b)));
+  constexpr bool kExact = !kBias && sizeof(T) == 2;
+  const uint32_t reach = kBias ? (p.sigmoid ? kNearSigmoid : kNearSoftmax) : 0;
+  // whether b, which comes after a in the order, may belong before it
+  auto near = [&](uint32_t a, uint32_t b) {
+    return !kExact && (a >> kIdBits) - (b >> kIdBits) <= reach;
   };
   bool plain = false;  // this token goes the plain way
 
   if (p.groups > 1) {
-    // the group's value on its lanes: the best choice, or the sum of the two best
-    uint32_t gkey;
-    const bool sums = p.group_top2;
-    {
-      uint32_t best = 0, second = 0;
+    const int group = sub / group_lanes;
+    uint32_t value;  // the group's, on its lanes, made unique by its number
+    if (!sums) {
+      value = key[0];
+#pragma unroll
+      for (int i = 1; i < kPer; ++i) value = max(value, key[i]);
+      for (int o = 1; o < group_lanes; o <<= 1)
+        value = max(value, __shfl_xor_sync(~0u, value, o));
+    } else {
+      uint32_t a = 0, b = 0;  // the two best of the codes, or of the logits
+      float fa = -INFINITY, fb = -INFINITY;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        second = max(second, min(best, key[i]));
-        best = max(best, key[i]);
+        if constexpr (kBias) {
+          b = max(b, min(a, key[i]));
+          a = max(a, key[i]);
+        } else {
+          const float y = masked(v[i]);
+          fb = fmaxf(fb, fminf(fa, y));
+          fa = fmaxf(fa, y);
+        }
       }
       for (int o = 1; o < group_lanes; o <<= 1) {
-        const uint32_t b2 = __shfl_xor_sync(~0u, best, o), s2 = __shfl_xor_sync(~0u, second, o);
-        second = max(min(best, b2), max(second, s2));
-        best = max(best, b2);
+        if constexpr (kBias) {
+          const uint32_t a2 = __shfl_xor_sync(~0u, a, o), b2 = __shfl_xor_sync(~0u, b, o);
+          b = max(min(a, a2), max(b, b2));
+          a = max(a, a2);
+        } else {
+          const float a2 = __shfl_xor_sync(~0u, fa, o), b2 = __shfl_xor_sync(~0u, fb, o);
+          fb = fmaxf(fminf(fa, a2), fmaxf(fb, b2));
+          fa = fmaxf(fa, a2);
+        }
       }
-      if (sums && best) {
-        auto value = [&](uint32_t key) {
-          const float c = keys::order_value(key);
-          return p.bias ? c : score(c);
-        };
-        gkey = choice_key(second ? value(best) + value(second) : value(best));
+      // their sum in units of 2^-20, from 0 up
+      constexpr uint32_t kZero = kFixedZero >> kDrop;
+      if constexpr (kBias) {
+        value = (1u << 24) + (a >> kIdBits) - kZero + (b ? (b >> kIdBits) - kZero : 0);
+        if (!a) value = 0;
       } else {
-        gkey = best;
+        value = (1u << 24) + fixed_code(score(fa)) - kFixedZero +
+                (fb > -INFINITY ? fixed_code(score(fb)) - kFixedZero : 0);
+        if (!(fa > -INFINITY)) value = 0;
       }
+      value = value ? value << 5 | (31 - group) : 0;
     }
-    // stands: how many groups are better (equal ones: lower) is below topk_groups
-    uint32_t left = gkey, last = 0;
-    bool open = false;
+    uint32_t left = value, last = 0;
     for (int i = 0; i < p.topk_groups; ++i) {
       const uint32_t big = lanes_max<kLanes>(left);
-      const unsigned who = __ballot_sync(~0u, left == big && big) & mine;
-      if (who && sub / group_lanes == (__ffs(who) - 1) % kLanes / group_lanes) {
-        open = true;
-        left = 0;
-      }
+      left = left == big ? 0 : left;
       last = big;
     }
-    if (sums || p.bias) {  // in doubt: the best group that fell, near the last that stands
-      const uint32_t fell = lanes_max<kLanes>(left);
-      const float a = keys::order_value(last), b = keys::order_value(fell);
-      plain = last && fell && near(sums ? 0.5f * a : a, sums ? 0.5f * b : b);
+    const uint32_t fell = lanes_max<kLanes>(left);
+    if (last && fell) {
+      if (sums) {
+        const uint32_t far = 2 * (p.sigmoid ? kNearSigmoid : kNearSoftmax) + 2;
+        plain = (last >> 5) - (fell >> 5) <= far;
+      } else {
+        plain = near(last, fell);
+      }
     }
-    if (!open) {
+    if (left) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) key[i] = 0;
     }
   }
 
-  // The k best, one at a time (with a bias also the one after them), on lanes 0.. of the token:
-  // slot j of lane s is number j * kLanes + s.
+  // The k best, one at a time, and the one after them if it could be in doubt. Slot j of lane s
+  // of the token holds number j * kLanes + s.
   constexpr int kSlots = 32 / kLanes;
   int id[kSlots];
-  uint32_t at[kSlots];
+  uint32_t at[kSlots], previous = 0;
 #pragma unroll
   for (int j = 0; j < kSlots; ++j) {
     id[j] = -1;
     at[j] = 0;
   }
+  bool doubt = false;
   uint32_t best = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) best = max(best, key[i]);
-  int next_id = -1;
-  uint32_t next_key = 0;
-  const int rounds = p.bias ? k + 1 : k;
-  for (int r = 0; r < rounds; ++r) {
+  for (int r = 0; r < (kExact ? k : k + 1); ++r) {
     const uint32_t big = lanes_max<kLanes>(best);
-    const unsigned who = __ballot_sync(~0u, best == big) & mine;
-    const int from = __ffs(who) - 1;
-    int e = 0;
-    if (lane == from && big) {
-      bool found = false;
+    doubt = doubt || (r && big && near(previous, big));
+    previous = big;
+    if (r == k) break;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const bool hit = !found && key[i] == big;
-        found = found || hit;
-        e = hit ? i : e;
-        if (hit && r < k) key[i] = 0;
+    for (int j = 0; j < kSlots; ++j) {
+      if (j * kLanes + sub == r && big) {
+        id[j] = static_cast<int>(kIds - (big & kIds));
+        at[j] = big;
       }
-      best = 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) best = max(best, key[i]);
     }
-    e = __shfl_sync(~0u, e, from) + from % kLanes * kPer;
-    if (r < k) {
+    best = 0;
 #pragma unroll
-      for (int j = 0; j < kSlots; ++j) {
-        if (j * kLanes + sub == r && big) {
-          id[j] = e;
-          at[j] = big;
-        }
-      }
-    } else if (big) {
-      next_id = e;
-      next_key = big;
+    for (int i = 0; i < kPer; ++i) {
+      key[i] = key[i] == big ? 0 : key[i];
+      best = max(best, key[i]);
     }
   }
 
-  if (p.bias) {
+  if (!kExact && __any_sync(~0u, doubt && live && !plain)) {
     // Neighbours in the order that stand too near: settled if they are equal in logit and bias
     // (lower ids come first); the k-th and what is left have to be clear apart. Else 64 bits
     // decide.
-    bool in_doubt = false;
+    const int next_id = static_cast<int>(kIds - (previous & kIds));
+    bool open = false;
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
       const int r = j * kLanes + sub;
+      constexpr int kLast = kSlots - 1;
       int i2 = __shfl_down_sync(~0u, id[j], 1, kLanes);
       uint32_t k2 = __shfl_down_sync(~0u, at[j], 1, kLanes);
-      const int i3 = j + 1 < kSlots ? __shfl_sync(~0u, id[j + 1 < kSlots ? j + 1 : j], 0, kLanes) : -1;
-      const uint32_t k3 = j + 1 < kSlots ? __shfl_sync(~0u, at[j + 1 < kSlots ? j + 1 : j], 0, kLanes) : 0;
+      const int i3 = __shfl_sync(~0u, id[j < kLast ? j + 1 : j], 0, kLanes);
+      const uint32_t k3 = __shfl_sync(~0u, at[j < kLast ? j + 1 : j], 0, kLanes);
       if (sub == kLanes - 1) {
-        i2 = i3;
-        k2 = k3;
+        i2 = j < kLast ? i3 : -1;
+        k2 = j < kLast ? k3 : 0;
       }
       if (r == k - 1) {
         i2 = next_id;
-        k2 = next_key;
+        k2 = previous;
       }
-      if (r < k && at[j] && k2 && near(keys::order_value(at[j]), keys::order_value(k2))) {
-        const float xa = score_f32(x[id[j]]), xb = score_f32(x[i2]);
-        const bool settled = r < k - 1 && __ldg(p.bias + id[j]) == __ldg(p.bias + i2) &&
-                             xa == xb && id[j] < i2;
-        in_doubt = in_doubt || !settled;
+      if (r < k && at[j] && k2 && near(at[j], k2)) {
+        const bool equal = score_f32(x[id[j]]) == score_f32(x[i2]) &&
+                           (!kBias || __ldg(p.bias + id[j]) == __ldg(p.bias + i2));
+        open = open || !(r < k - 1 && equal);
       }
     }
-    in_doubt = __ballot_sync(~0u, in_doubt) & mine;
-    unsigned todo = __ballot_sync(~0u, in_doubt && live && !plain && sub == 0);
+    open = __ballot_sync(~0u, open) & mine;
+    unsigned todo = __ballot_sync(~0u, open && live && !plain && sub == 0);
     while (todo) {  // one token at a time, by the whole warp
-      const int lead = __ffs(todo) - 1, first = lead, slot0 = lead / kLanes;
+      const int first = __ffs(todo) - 1, slot0 = first / kLanes;
       todo &= todo - 1;
       const T* xt = static_cast<const T*>(p.logits) + (t0 + slot0) * p.ld;
       const bool here = lane / kLanes == slot0;
@@ -471,10 +492,9 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
         count += __popc(who);
       }
       if (cut) {
-        const float least = keys::order_value(cut);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-          const bool in = here && key[i] && near(least, keys::order_value(key[i]));
+          const bool in = here && key[i] && near(cut, key[i]);
           const unsigned who = __ballot_sync(~0u, in);
           const int place = count + __popc(who & ((1u << lane) - 1));
           if (in && place < 32) ids_of[warp][place] = e0 + i;
@@ -487,7 +507,7 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
       }
       __syncwarp();
       double md = -INFINITY, z = 1.0;
-      if (!p.sigmoid) {
+      if (kBias && !p.sigmoid) {
         float mf = -INFINITY;
         for (int e = lane; e < n; e += 32) mf = fmaxf(mf, masked(score_f32(xt[e])));
         mf = lanes_max<32>(mf);
@@ -503,10 +523,11 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
       double c = -INFINITY;
       if (lane < count) {
         e = ids_of[warp][lane];
-        const float y = score_f32(xt[e]);
-        const double s = p.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(y)))
-                                   : (y == md ? 1.0 : exp(static_cast<double>(y) - md)) / z;
-        c = s + static_cast<double>(__ldg(p.bias + e));
+        c = score_f32(xt[e]);
+        if constexpr (kBias) {
+          const double s = p.sigmoid ? 1.0 / (1.0 + exp(-c)) : (c == md ? 1.0 : exp(c - md)) / z;
+          c = s + static_cast<double>(__ldg(p.bias + e));
+        }
       }
       int rank = 0;
       for (int l = 0; l < count; ++l) {
@@ -719,19 +740,20 @@ bool lines_up(const void* p, int64_t stride_bytes, size_t bytes) {
 
 template <class T, int kLanes, int kPer>
 cudaError_t route_fast(const RouteParams& p, int group_lanes, cudaStream_t stream) {
-  const bool whole = p.experts % kPer == 0 && lines_up(p.logits, p.ld * sizeof(T), 16);
-  const bool whole_scores = p.experts % kPer == 0 &&
-                            lines_up(p.scores, int64_t{p.experts} * sizeof(float), 16);
-  // the plain way's room: only a token whose groups or many experts are in doubt needs it
-  const size_t smem = p.bias || (p.groups > 1 && p.group_top2)
-                          ? static_cast<size_t>(kWarps) * 2 * p.experts * sizeof(double) : 0;
-  static std::atomic<uint64_t> done;
-  const cudaError_t e = allow_smem(route_kernel<T, kLanes, kPer>, 64 * 1024, done);
+  const bool cells = p.experts % kPer == 0;
+  const bool whole = cells && lines_up(p.logits, p.ld * sizeof(T), 16);
+  const bool whole_scores =
+      cells && lines_up(p.scores, int64_t{p.experts} * sizeof(float), 16) && lines_up(p.bias, 0, 16);
+  // the plain way's room, for a token whose groups or whose many experts are in doubt
+  const bool doubt = p.bias || sizeof(T) == 4 || (p.groups > 1 && p.group_top2);
+  const size_t smem = doubt ? static_cast<size_t>(kWarps) * 2 * p.experts * sizeof(double) : 0;
+  auto kernel = p.bias ? route_kernel<T, kLanes, kPer, true> : route_kernel<T, kLanes, kPer, false>;
+  static std::atomic<uint64_t> done[2];
+  const cudaError_t e = allow_smem(kernel, 64 * 1024, done[p.bias != nullptr]);
   if (e != cudaSuccess) return e;
   constexpr int kTokens = kWarps * 32 / kLanes;
-  route_kernel<T, kLanes, kPer>
-      <<<static_cast<unsigned>((p.tokens + kTokens - 1) / kTokens), kThreads, smem, stream>>>(
-          p, group_lanes, whole, whole_scores);
+  kernel<<<static_cast<unsigned>((p.tokens + kTokens - 1) / kTokens), kThreads, smem, stream>>>(
+      p, group_lanes, whole, whole_scores);
   return cudaGetLastError();
 }
 
