@@ -106,7 +106,7 @@ __device__ __forceinline__ float sigmoid_fast(float x) { return rcp_fast(1.f + e
 __device__ __forceinline__ float relative_score(float v, float top, bool sigmoid) {
   if (!sigmoid) return v == top ? 1.f : exp_fast(v - top);
   const float base = fminf(top, 0.f);
-  return 1.f / (exp_fast(base) + (v == base ? 1.f : exp_fast(base - v)));
+  return rcp_fast(exp_fast(base) + (v == base ? 1.f : exp_fast(base - v)));
 }
 
 // The plain way: one warp takes the token, choice and score of each expert in shared memory
@@ -304,7 +304,7 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
       z += v[i] > -INFINITY ? e : 0.f;
     }
     z = lanes_sum<kLanes>(z);
-    inv_z = z > 0.f ? 1.f / z : 0.f;
+    inv_z = z > 0.f ? rcp_fast(z) : 0.f;
   }
   auto score = [&](float y) {
     const float s = p.sigmoid ? sigmoid_fast(y) : (y == m ? 1.f : exp_fast(y - m)) * inv_z;
@@ -421,23 +421,74 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
   uint32_t best = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) best = max(best, key[i]);
-  for (int r = 0; r < (kExact ? k : k + 1); ++r) {
-    const uint32_t big = lanes_max<kLanes>(best);
-    doubt = doubt || (r && big && near(previous, big));
-    previous = big;
-    if (r == k) break;
-#pragma unroll
-    for (int j = 0; j < kSlots; ++j) {
-      if (j * kLanes + sub == r && big) {
-        id[j] = static_cast<int>(kIds - (big & kIds));
-        at[j] = big;
-      }
+  const int wanted = kExact ? k : k + 1;
+  bool listed = false;
+  if constexpr (kLanes == 32) {
+    // With a whole warp a token: the wanted-th largest of the lanes' bests bounds the wanted-th
+    // key from below, and the few keys that reach it (13 on average for 9 of 256) are ranked
+    // against one another, a lane each. Where more than a warp's lanes reach it they are taken
+    // out one by one, as for smaller tokens.
+    uint32_t left = best, bound = 0;
+    for (int r = 0; r < wanted; ++r) {
+      bound = __reduce_max_sync(~0u, left);
+      left = left == bound ? 0 : left;
     }
-    best = 0;
+    bound = max(bound, 1u);
+    int count = 0;
+    uint32_t* keys_of = reinterpret_cast<uint32_t*>(ids_of[warp]);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      key[i] = key[i] == big ? 0 : key[i];
-      best = max(best, key[i]);
+      const bool in = key[i] >= bound;
+      const unsigned who = __ballot_sync(~0u, in);
+      const int place = count + __popc(who & ((1u << lane) - 1));
+      if (in && place < 32) keys_of[place] = key[i];
+      count += __popc(who);
+    }
+    listed = count <= 32;
+    if (listed) {
+      __syncwarp();
+      const uint32_t own = lane < count ? keys_of[lane] : 0;
+      int rank = 0;
+      for (int l = 0; l < count; ++l) rank += keys_of[l] > own;
+      __syncwarp();
+      if (lane < count) keys_of[rank] = own;
+      __syncwarp();
+      const uint32_t big = lane < count ? keys_of[lane] : 0;
+      const uint32_t after = __shfl_down_sync(~0u, big, 1);
+      doubt = __any_sync(~0u, lane < 31 && lane < wanted - 1 && after && near(big, after));
+      previous = __shfl_sync(~0u, big, min(wanted - 1, 31));
+      if (wanted > 32) previous = 0;
+      if (lane < k) {
+        id[0] = big ? static_cast<int>(kIds - (big & kIds)) : -1;
+        at[0] = big;
+      }
+      if (!kExact && doubt) {  // what is left, for the candidates below
+        const uint32_t last = __shfl_sync(~0u, big, k - 1);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) key[i] = key[i] >= last ? 0 : key[i];
+      }
+    }
+    __syncwarp();
+  }
+  if (!listed) {
+    for (int r = 0; r < wanted; ++r) {
+      const uint32_t big = lanes_max<kLanes>(best);
+      doubt = doubt || (r && big && near(previous, big));
+      previous = big;
+      if (r == k) break;
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j) {
+        if (j * kLanes + sub == r && big) {
+          id[j] = static_cast<int>(kIds - (big & kIds));
+          at[j] = big;
+        }
+      }
+      best = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        key[i] = key[i] == big ? 0 : key[i];
+        best = max(best, key[i]);
+      }
     }
   }
 
@@ -564,9 +615,10 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
       w[j] = id[j] >= 0 ? relative_score(y[j], top, p.sigmoid) : 0.f;
       total += w[j];
     }
-    total = lanes_sum<kLanes>(total);
+    total = lanes_sum<kLanes>(total);  // 0, or at least a half
+    const float inv = total > 0.f ? rcp_fast(total) : 0.f;
 #pragma unroll
-    for (int j = 0; j < kSlots; ++j) w[j] = total > 0.f ? w[j] / total : 0.f;
+    for (int j = 0; j < kSlots; ++j) w[j] *= inv;
   } else {
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) w[j] = score(y[j]);
@@ -654,7 +706,7 @@ route_backward_kernel(RouteBackwardParams p, bool whole, bool whole_out, bool wh
         z += v[i];
       }
       z = lanes_sum<kLanes>(z);
-      inv_z = z > 0.f ? 1.f / z : 0.f;
+      inv_z = z > 0.f ? rcp_fast(z) : 0.f;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) v[i] *= inv_z;  // the scores from here on
     }
@@ -669,10 +721,11 @@ route_backward_kernel(RouteBackwardParams p, bool whole, bool whole_out, bool wh
       own[j] = id[j] >= 0 ? relative_score(y[j], top, p.sigmoid) : 0.f;
       total += own[j];
     }
-    total = lanes_sum<kLanes>(total);
+    total = lanes_sum<kLanes>(total);  // 0, or at least a half
+    const float inv = total > 0.f ? rcp_fast(total) : 0.f;
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
-      own[j] = total > 0.f ? own[j] / total : 0.f;
+      own[j] *= inv;
       mean += own[j] * dw[j];
     }
     mean = lanes_sum<kLanes>(mean);
@@ -696,19 +749,29 @@ route_backward_kernel(RouteBackwardParams p, bool whole, bool whole_out, bool wh
     for (int i = 0; i < kPer; ++i) dot += v[i] * d[i];
     dot = lanes_sum<kLanes>(dot);
   }
-  // the parts at their places, added in order where an expert stands twice
+  // The parts at their places. Each lane writes its own where no expert stands twice for a token
+  // (which shows when every lane finds its own mark again); else one lane adds them in order.
   float4* cells = reinterpret_cast<float4*>(part + e0);
 #pragma unroll
   for (int i = 0; i < kPer / 4; ++i) cells[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-  for (int j = 0; j < kSlots; ++j) {
-    own_of[j * kLanes + sub] = own[j];
-    id_of[j * kLanes + sub] = id[j];
-  }
   __syncwarp();
-  if (sub == 0) {
-    for (int r = 0; r < k; ++r)
-      if (id_of[r] >= 0) part[id_of[r]] += own_of[r];
+  if (id[0] >= 0) part[id[0]] = __int_as_float(lane);
+  __syncwarp();
+  const bool alone = id[0] < 0 || __float_as_int(part[id[0]]) == lane;
+  if (__all_sync(~0u, alone && k <= kLanes)) {
+    if (id[0] >= 0) part[id[0]] = own[0];
+  } else {
+    if (id[0] >= 0) part[id[0]] = 0.f;
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      own_of[j * kLanes + sub] = own[j];
+      id_of[j * kLanes + sub] = id[j];
+    }
+    __syncwarp();
+    if (sub == 0) {
+      for (int r = 0; r < k; ++r)
+        if (id_of[r] >= 0) part[id_of[r]] += own_of[r];
+    }
   }
   __syncwarp();
   float g[kPer];

@@ -3,9 +3,9 @@
 // pairs of its expert in earlier warps + those before it in its own warp.
 //
 // Up to kSmall pairs one block does it all (one launch: 4.8 us for 512 pairs of 256 experts).
-// Beyond that up to kMostBlocks blocks of kBlockPairs or more pairs work side by side, in three
-// launches with no workspace: the blocks' counts wait in `position`, whose own contents come
-// last, from `order`.
+// Beyond that up to kMostBlocks blocks of kBlockPairs or more pairs work side by side, in four
+// launches with no workspace: the blocks' counts wait in `position` and the experts' in `offsets`,
+// whose own contents come last.
 #include "rows.cuh"
 
 namespace ovvs {
@@ -16,8 +16,17 @@ constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kSmall = 4096;
 constexpr int kBlockPairs = 4096;  // and multiples of it
-constexpr int kMostBlocks = 512;   // every block reads all blocks' counts
+constexpr int kMostBlocks = 512;
 static_assert(kBlockPairs >= kRouteMaxExperts, "position holds a count per block and expert");
+
+// The launches of a large plan follow one another closely: each says at once that the next may
+// be set up, and waits for the one before it to have finished before it reads what that wrote.
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_last() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
 __device__ __forceinline__ int expert_of(const int* ids, int64_t i, int64_t end, int experts) {
   const int e = i < end ? __ldg(ids + i) : -1;
@@ -48,6 +57,19 @@ __device__ __forceinline__ int block_scan(int v, int* buf, int* all) {
 }
 static_assert(kWarps == 32, "one total a lane");
 
+// The lanes that hold the same e, for e in [-1, 2^bits): one vote a bit. (__match_any_sync takes
+// longer the more values there are, some 60 cycles of the SM here.)
+__device__ __forceinline__ unsigned same_expert(int e, int bits) {
+  const unsigned there = __ballot_sync(~0u, e >= 0);
+  unsigned same = e >= 0 ? there : ~there;
+  for (int b = 0; b < bits; ++b) {
+    const bool one = e >> b & 1;
+    const unsigned ones = __ballot_sync(~0u, one);
+    same &= one ? ones : ~ones;
+  }
+  return same;
+}
+
 // counts[warp][expert] of the pairs [i0, i1) of each warp.
 __device__ __forceinline__ void count_pairs(const int* ids, int64_t i0, int64_t i1, int experts,
                                             int* counts) {
@@ -55,6 +77,7 @@ __device__ __forceinline__ void count_pairs(const int* ids, int64_t i0, int64_t 
   for (int i = threadIdx.x; i < kWarps * experts; i += kThreads) counts[i] = 0;
   __syncthreads();
   int* own = counts + (threadIdx.x >> 5) * experts;
+#pragma unroll 4
   for (int64_t i = i0 + lane; i < i1; i += 32) {
     const int e = expert_of(ids, i, i1, experts);
     if (e >= 0) atomicAdd(own + e, 1);
@@ -68,18 +91,26 @@ __device__ __forceinline__ void place_pairs(const int* ids, int64_t i0, int64_t 
                                             int* counts, int* order, int* position) {
   const int lane = threadIdx.x & 31;
   int* own = counts + (threadIdx.x >> 5) * experts;
-  for (int64_t b = i0; b < i1; b += 32) {
-    const int64_t i = b + lane;
-    const int e = expert_of(ids, i, i1, experts);
-    const unsigned same = __match_any_sync(~0u, e);
-    int at = -1;
-    if (e >= 0) at = own[e] + __popc(same & ((1u << lane) - 1));
-    __syncwarp();
-    if (e >= 0 && lane == __ffs(same) - 1) own[e] += __popc(same);
-    __syncwarp();
-    if (i < i1) {
-      if (kPosition) position[i] = at;
-      if (at >= 0) order[at] = static_cast<int>(i);
+  constexpr int kAhead = 4;  // rows of ids under way at once
+  const int bits = 32 - __clz(experts - 1);
+  for (int64_t b = i0; b < i1; b += 32 * kAhead) {
+    int ahead[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) ahead[j] = expert_of(ids, b + j * 32 + lane, i1, experts);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int64_t i = b + j * 32 + lane;
+      const int e = ahead[j];
+      const unsigned same = same_expert(e, bits);
+      int at = -1;
+      if (e >= 0) at = own[e] + __popc(same & ((1u << lane) - 1));
+      __syncwarp();
+      if (e >= 0 && lane == __ffs(same) - 1) own[e] = at + __popc(same);
+      __syncwarp();
+      if (i < i1) {
+        if (kPosition) position[i] = at;
+        if (at >= 0) order[at] = static_cast<int>(i);
+      }
     }
   }
 }
@@ -118,10 +149,11 @@ route_plan_kernel(const int* ids, int64_t pairs, int experts, int align, int* of
   place_pairs<true>(ids, i0, i1, experts, counts, order, position);
 }
 
-// Large plans, first: the pairs of each expert in every block of pairs, to table[block][expert].
+// Large plans, first: the pairs of each expert in every block of pairs, to table[expert][block].
 __global__ void __launch_bounds__(kThreads)
 plan_count_kernel(const int* ids, int64_t pairs, int64_t block_pairs, int experts, int* table) {
   extern __shared__ int counts[];  // [experts]
+  let_next_start();
   for (int e = threadIdx.x; e < experts; e += kThreads) counts[e] = 0;
   __syncthreads();
   const int64_t b = blockIdx.x * block_pairs;
@@ -133,60 +165,57 @@ plan_count_kernel(const int* ids, int64_t pairs, int64_t block_pairs, int expert
   }
   __syncthreads();
   for (int e = threadIdx.x; e < experts; e += kThreads)
-    table[static_cast<int64_t>(blockIdx.x) * experts + e] = counts[e];
+    table[e * static_cast<int>(gridDim.x) + blockIdx.x] = counts[e];
 }
 
-// Second: every block sums the table for itself (the whole of it, from L2), which gives the
-// segments and where its own pairs start in them, and puts its pairs in order.
+// Second: a warp an expert; running sums over the blocks, in place, and the total.
+__global__ void __launch_bounds__(kThreads)
+plan_sum_kernel(int experts, int blocks, int* table, int* totals) {
+  const int lane = threadIdx.x & 31;
+  const int e = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  let_next_start();
+  wait_for_last();
+  if (e >= experts) return;
+  int* row = table + e * blocks;
+  constexpr int kPer = kMostBlocks / 32;
+  int c[kPer], run = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) c[j] = j * 32 + lane < blocks ? row[j * 32 + lane] : 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    if (j * 32 >= blocks) break;
+    int s = c[j];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(~0u, s, o);
+      if (lane >= o) s += y;
+    }
+    if (j * 32 + lane < blocks) row[j * 32 + lane] = run + s - c[j];
+    run += __shfl_sync(~0u, s, 31);
+  }
+  if (lane == 0) totals[e] = run;
+}
+
+// Third: every block puts its pairs in order.
 __global__ void __launch_bounds__(kThreads)
 plan_order_kernel(const int* ids, int64_t pairs, int64_t block_pairs, int experts, int align,
-                  const int* table, int* offsets, int* order, int64_t capacity) {
+                  const int* table, const int* totals, int* order, int64_t capacity) {
   extern __shared__ int counts[];  // [kWarps][experts]
   __shared__ int buf[kWarps];
   const int tid = threadIdx.x, warp = tid >> 5;
   const int blocks = gridDim.x, block = blockIdx.x;
-  // `parts` threads an expert, each over every parts-th block: (pairs before this block, in all)
-  int parts = 1;
-  while (parts * 2 * experts <= kThreads) parts *= 2;
-  const int e = tid / parts, part = tid % parts;
-  int before = 0, total = 0;
-  if (e < experts) {
-#pragma unroll 8
-    for (int b = part; b < blocks; b += parts) {
-      const int c = __ldg(table + static_cast<int64_t>(b) * experts + e);
-      total += c;
-      before += b < block ? c : 0;
-    }
-  }
-  // parts is a power of two, but may be more than a warp's lanes: joined in shared memory
-  for (int i = tid; i < 2 * experts; i += kThreads) counts[i] = 0;
-  __syncthreads();
-  if (e < experts) {
-    atomicAdd(&counts[e], total);
-    atomicAdd(&counts[experts + e], before);
-  }
-  __syncthreads();
-  total = tid < experts ? counts[tid] : 0;
-  before = tid < experts ? counts[experts + tid] : 0;
-  __syncthreads();
-  const int padded = (total + align - 1) / align * align;
-  int all;
-  const int first = block_scan(padded, buf, &all);
-  if (tid < experts) {
-    if (block == 0) {
-      offsets[tid] = first;
-      if (tid == experts - 1) offsets[experts] = all;
-    }
-    if (tid % blocks == block)
-      for (int i = total; i < padded; ++i) order[first + i] = -1;
-  }
-  for (int64_t i = all + static_cast<int64_t>(block) * kThreads + tid; i < capacity;
-       i += static_cast<int64_t>(blocks) * kThreads)
-    order[i] = -1;
+  let_next_start();
   const int64_t span = block_pairs / kWarps;
   const int64_t i0 = block * block_pairs + warp * span;
   const int64_t i1 = i0 + span < pairs ? i0 + span : pairs;
   count_pairs(ids, i0, i1, experts, counts);
+  int* pad = counts + kWarps * experts;  // [2][experts]: where padding starts and ends
+  wait_for_last();
+  const int total = tid < experts ? __ldcg(totals + tid) : 0;
+  const int before = tid < experts ? __ldcg(table + tid * blocks + block) : 0;
+  const int padded = (total + align - 1) / align * align;
+  int all;
+  const int first = block_scan(padded, buf, &all);
   if (tid < experts) {
     int next = first + before;
 #pragma unroll 8
@@ -195,21 +224,57 @@ plan_order_kernel(const int* ids, int64_t pairs, int64_t block_pairs, int expert
       counts[w * experts + tid] = next;
       next += c;
     }
+    pad[tid] = first + total;
+    pad[experts + tid] = first + padded;
   }
   __syncthreads();
   place_pairs<false>(ids, i0, i1, experts, counts, order, nullptr);
+  for (int x = block; x < experts; x += blocks)
+    for (int i = pad[x] + tid; i < pad[experts + x]; i += kThreads) order[i] = -1;
+  for (int64_t i = all + static_cast<int64_t>(block) * kThreads + tid; i < capacity;
+       i += static_cast<int64_t>(blocks) * kThreads)
+    order[i] = -1;
 }
 
-// Third: position is the inverse of order; pairs without an expert have none.
-__global__ void __launch_bounds__(256)
-plan_position_kernel(const int* ids, int64_t pairs, int experts, const int* order,
-                     int64_t capacity, int* position) {
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
-  for (int64_t s = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; s < capacity; s += step) {
-    const int i = __ldg(order + s);
+// Last: position is the inverse of order, pairs without an expert have none; the totals become
+// the offsets.
+__global__ void __launch_bounds__(kThreads)
+plan_position_kernel(const int* ids, int64_t pairs, int experts, int align, const int* order,
+                     int64_t capacity, int* position, int* offsets) {
+  __shared__ int buf[kWarps];
+  const int tid = threadIdx.x;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+  wait_for_last();
+#pragma unroll 4
+  for (int64_t s = static_cast<int64_t>(blockIdx.x) * kThreads + tid; s < capacity; s += step) {
+    const int i = __ldcg(order + s);
     if (i >= 0) position[i] = static_cast<int>(s);
     if (s < pairs && expert_of(ids, s, pairs, experts) < 0) position[s] = -1;
   }
+  if (blockIdx.x == 0) {
+    const int total = tid < experts ? offsets[tid] : 0;
+    int all;
+    const int first = block_scan((total + align - 1) / align * align, buf, &all);
+    if (tid < experts) offsets[tid] = first;
+    if (tid == 0) offsets[experts] = all;
+  }
+}
+
+// A launch that may be set up while the one before it on the stream still runs.
+template <class... P, class... A>
+cudaError_t launch_after(void (*kernel)(P...), unsigned blocks, int threads, size_t smem,
+                         cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
 }  // namespace
@@ -218,7 +283,7 @@ cudaError_t launch_route_plan(const int* ids, int64_t pairs, int experts, int al
                               int* offsets, int* order, int64_t capacity, int* position,
                               cudaStream_t stream) {
   const int smem = kWarps * experts * static_cast<int>(sizeof(int));
-  constexpr int kMost = kWarps * kRouteMaxExperts * static_cast<int>(sizeof(int));
+  constexpr int kMost = (kWarps + 2) * kRouteMaxExperts * static_cast<int>(sizeof(int));
   if (pairs <= kSmall) {
     static std::atomic<uint64_t> done;
     const cudaError_t e = allow_smem(route_plan_kernel, kMost, done);
@@ -228,18 +293,24 @@ cudaError_t launch_route_plan(const int* ids, int64_t pairs, int experts, int al
     return cudaGetLastError();
   }
   static std::atomic<uint64_t> done;
-  const cudaError_t e = allow_smem(plan_order_kernel, kMost, done);
+  cudaError_t e = allow_smem(plan_order_kernel, kMost, done);
   if (e != cudaSuccess) return e;
   const int64_t units = (pairs + kBlockPairs - 1) / kBlockPairs;
   const int64_t block_pairs = (units + kMostBlocks - 1) / kMostBlocks * kBlockPairs;
   const unsigned blocks = static_cast<unsigned>((pairs + block_pairs - 1) / block_pairs);
+  const int64_t sweep = (capacity + 2 * kThreads - 1) / (2 * kThreads);
+  const unsigned sweep_blocks = static_cast<unsigned>(sweep < 296 ? sweep : 296);
   plan_count_kernel<<<blocks, kThreads, experts * sizeof(int), stream>>>(ids, pairs, block_pairs,
                                                                          experts, position);
-  plan_order_kernel<<<blocks, kThreads, smem, stream>>>(ids, pairs, block_pairs, experts, align,
-                                                        position, offsets, order, capacity);
-  const int64_t sweep = (capacity + 255) / 256;
-  plan_position_kernel<<<static_cast<unsigned>(sweep < 148 * 8 ? sweep : 148 * 8), 256, 0,
-                         stream>>>(ids, pairs, experts, order, capacity, position);
+  e = launch_after(plan_sum_kernel, (experts + kWarps - 1) / kWarps, kThreads, 0, stream, experts,
+                   static_cast<int>(blocks), position, offsets);
+  if (e != cudaSuccess) return e;
+  e = launch_after(plan_order_kernel, blocks, kThreads, smem + 2 * experts * sizeof(int), stream,
+                   ids, pairs, block_pairs, experts, align, position, offsets, order, capacity);
+  if (e != cudaSuccess) return e;
+  e = launch_after(plan_position_kernel, sweep_blocks, kThreads, 0, stream, ids, pairs, experts,
+                   align, order, capacity, position, offsets);
+  if (e != cudaSuccess) return e;
   return cudaGetLastError();
 }
 
