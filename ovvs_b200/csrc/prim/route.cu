@@ -815,9 +815,8 @@ cudaError_t route_fast(const RouteParams& p, int group_lanes, cudaStream_t strea
   const cudaError_t e = allow_smem(kernel, 64 * 1024, done[p.bias != nullptr]);
   if (e != cudaSuccess) return e;
   constexpr int kTokens = kWarps * 32 / kLanes;
-  kernel<<<static_cast<unsigned>((p.tokens + kTokens - 1) / kTokens), kThreads, smem, stream>>>(
-      p, group_lanes, whole, whole_scores);
-  return cudaGetLastError();
+  const LaunchShape shape{static_cast<unsigned>((p.tokens + kTokens - 1) / kTokens), kThreads, smem};
+  return launch(kernel, shape, stream, p, group_lanes, whole, whole_scores);
 }
 
 template <class T>
@@ -839,9 +838,8 @@ cudaError_t route(const RouteParams& p, cudaStream_t stream) {
   static std::atomic<uint64_t> done;
   const cudaError_t e = allow_smem(route_plain_kernel<T>, 64 * 1024, done);
   if (e != cudaSuccess) return e;
-  route_plain_kernel<T><<<static_cast<unsigned>((p.tokens + kWarps - 1) / kWarps), kThreads, smem,
-                          stream>>>(p);
-  return cudaGetLastError();
+  const LaunchShape shape{static_cast<unsigned>((p.tokens + kWarps - 1) / kWarps), kThreads, smem};
+  return launch(route_plain_kernel<T>, shape, stream, p);
 }
 
 template <class T, int kLanes, int kPer>
@@ -853,10 +851,9 @@ cudaError_t route_backward_as(const RouteBackwardParams& p, cudaStream_t stream)
   constexpr int kTokens = kWarps * 32 / kLanes;
   constexpr size_t smem = static_cast<size_t>(kTokens) * (kLanes * kPer + 64) * sizeof(float);
   static_assert(smem <= 48 * 1024, "no opt-in needed");
-  route_backward_kernel<T, kLanes, kPer>
-      <<<static_cast<unsigned>((p.tokens + kTokens - 1) / kTokens), kThreads, smem, stream>>>(
-          p, whole, whole_out, whole_scores);
-  return cudaGetLastError();
+  const LaunchShape shape{static_cast<unsigned>((p.tokens + kTokens - 1) / kTokens), kThreads, smem};
+  return launch(route_backward_kernel<T, kLanes, kPer>, shape, stream, p, whole, whole_out,
+                whole_scores);
 }
 
 template <class T>

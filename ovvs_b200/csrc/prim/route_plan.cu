@@ -260,23 +260,6 @@ plan_position_kernel(const int* ids, int64_t pairs, int experts, int align, cons
   }
 }
 
-// A launch that may be set up while the one before it on the stream still runs.
-template <class... P, class... A>
-cudaError_t launch_after(void (*kernel)(P...), unsigned blocks, int threads, size_t smem,
-                         cudaStream_t stream, A... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
-}
-
 }  // namespace
 
 cudaError_t launch_route_plan(const int* ids, int64_t pairs, int experts, int align,
@@ -288,9 +271,8 @@ cudaError_t launch_route_plan(const int* ids, int64_t pairs, int experts, int al
     static std::atomic<uint64_t> done;
     const cudaError_t e = allow_smem(route_plan_kernel, kMost, done);
     if (e != cudaSuccess) return e;
-    route_plan_kernel<<<1, kThreads, smem, stream>>>(ids, pairs, experts, align, offsets, order,
-                                                     capacity, position);
-    return cudaGetLastError();
+    return launch(route_plan_kernel, {1, kThreads, static_cast<size_t>(smem)}, stream, ids, pairs,
+                  experts, align, offsets, order, capacity, position);
   }
   static std::atomic<uint64_t> done;
   cudaError_t e = allow_smem(plan_order_kernel, kMost, done);
@@ -300,18 +282,20 @@ cudaError_t launch_route_plan(const int* ids, int64_t pairs, int experts, int al
   const unsigned blocks = static_cast<unsigned>((pairs + block_pairs - 1) / block_pairs);
   const int64_t sweep = (capacity + 2 * kThreads - 1) / (2 * kThreads);
   const unsigned sweep_blocks = static_cast<unsigned>(sweep < 296 ? sweep : 296);
-  plan_count_kernel<<<blocks, kThreads, experts * sizeof(int), stream>>>(ids, pairs, block_pairs,
-                                                                         experts, position);
-  e = launch_after(plan_sum_kernel, (experts + kWarps - 1) / kWarps, kThreads, 0, stream, experts,
-                   static_cast<int>(blocks), position, offsets);
+  const unsigned sum_blocks = static_cast<unsigned>((experts + kWarps - 1) / kWarps);
+  LaunchShape shape{blocks, kThreads, experts * sizeof(int)};
+  e = launch(plan_count_kernel, shape, stream, ids, pairs, block_pairs, experts, position);
   if (e != cudaSuccess) return e;
-  e = launch_after(plan_order_kernel, blocks, kThreads, smem + 2 * experts * sizeof(int), stream,
-                   ids, pairs, block_pairs, experts, align, position, offsets, order, capacity);
+  shape = {sum_blocks, kThreads, 0, 1, true};
+  e = launch(plan_sum_kernel, shape, stream, experts, static_cast<int>(blocks), position, offsets);
   if (e != cudaSuccess) return e;
-  e = launch_after(plan_position_kernel, sweep_blocks, kThreads, 0, stream, ids, pairs, experts,
-                   align, order, capacity, position, offsets);
+  shape = {blocks, kThreads, smem + 2 * experts * sizeof(int), 1, true};
+  e = launch(plan_order_kernel, shape, stream, ids, pairs, block_pairs, experts, align, position,
+             offsets, order, capacity);
   if (e != cudaSuccess) return e;
-  return cudaGetLastError();
+  shape = {sweep_blocks, kThreads, 0, 1, true};
+  return launch(plan_position_kernel, shape, stream, ids, pairs, experts, align, order, capacity,
+                position, offsets);
 }
 
 }  // namespace prim

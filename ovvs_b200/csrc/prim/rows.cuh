@@ -31,6 +31,39 @@ inline cudaError_t allow_smem(Kernel* kernel, int bytes, std::atomic<uint64_t>& 
   return e;
 }
 
+// One launch; the status is its own. `cluster`: blocks a cluster; `follows`: it may be set up while
+// the kernel before it on the stream still runs (and waits for that one itself).
+struct LaunchShape {
+  unsigned blocks;
+  int threads;
+  size_t smem = 0;
+  unsigned cluster = 1;
+  bool follows = false;
+};
+template <class... P, class... A>
+cudaError_t launch(void (*kernel)(P...), const LaunchShape& shape, cudaStream_t stream,
+                   A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(shape.blocks);
+  cfg.blockDim = dim3(static_cast<unsigned>(shape.threads));
+  cfg.dynamicSmemBytes = shape.smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2]{};
+  if (shape.cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = shape.cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (shape.follows) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  cfg.attrs = attr;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // ovvsScoreType (ovvs_cuda.h).
 enum ScoreType : int { kScoreF32 = 0, kScoreF16 = 1, kScoreBf16 = 16 };
 

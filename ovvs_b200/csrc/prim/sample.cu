@@ -879,27 +879,37 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     return warp_reduce((lane < me ? a : 0) + (32 + lane < me ? b : 0), Add());
   };
   // Edge of the shortest prefix, among the columns up to `in`, whose sum of value(x) reaches
-  // target: the score one 8-bit digit at a time, then the column among those that share it.
-  auto reach = [&](u64 in, u64 target, auto&& value) {
+  // target, where the scores from `high` on sum to `above` and it ends among those below from
+  // `low` on (0 if it does not): the score one 8-bit digit at a time, then the column among those
+  // that share it.
+  auto reach = [&](u64 in, u64 target, u64 above, float low, float high, auto&& value) -> u64 {
     u64* hist = sh.wts;
-    u64 above = 0;
     uint32_t prefix = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
       cluster.sync();
       hist[tid] = 0;
       __syncthreads();
       const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
+      uint32_t at = 0;  // equal scores in a row are added up before they go to their bin
+      u64 sum = 0;
       each([&](float y, int col) {
+        if (!(y >= low) || y >= high) return;
         const uint32_t k = sort_key(y);
-        if (k && (k & mask) == prefix && element(k, col) >= in) {
-          const u64 v = value(y);
-          if (v) atomicAdd(&hist[(k >> shift) & 255], v);
+        if ((k & mask) != prefix || element(k, col) < in) return;
+        const uint32_t bin = k >> shift & 255;
+        if (bin != at && sum) {
+          atomicAdd(&hist[at], sum);
+          sum = 0;
         }
+        at = bin;
+        sum += value(y);
       });
+      if (sum) atomicAdd(&hist[at], sum);
       cluster.sync();
       u64 bin = 0, all;
       for (int b = 0; b < nb; ++b) bin += cluster.map_shared_rank(hist, b)[255 - tid];
       const u64 before = above + block_scan(bin, sh.red, &all);
+      if (above >= target || above + all < target) return 0;
       if (before < target && before + bin >= target) {
         sh.pick = 255 - tid;
         sh.above = before;
@@ -926,6 +936,8 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     return element(prefix, static_cast<uint32_t>(sh.found));
   };
 
+  constexpr float kLowest = -3.402823466e38f;
+  const float none = __int_as_float(0x7fffffff);  // no score reaches a NaN
   const u64 everything = element(1, ~0u);  // every column that is not masked
   u64 edge = everything;
   if (o.k > 0) {
@@ -933,7 +945,7 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     each([&](float y, int) { n += y > -INFINITY; });
     n = cluster_sum(n);
     if (static_cast<u64>(o.k) < n)
-      edge = reach(edge, static_cast<u64>(o.k), [](float) { return u64{1}; });
+      edge = reach(edge, static_cast<u64>(o.k), 0, kLowest, none, [](float) { return u64{1}; });
   }
   bool summed = false;  // tot holds the kept weights
   if (o.tp < 1.f) {
@@ -954,6 +966,7 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     __syncthreads();
     const float bins_f = binned ? static_cast<float>(kBins) : 0.f;
     const float unit_per_bin = 1.f / bins_per_unit;
+    float low = kLowest, high = none;
     u64 z = 0;
     auto weigh = [&](float y, bool in) {
       const u64 own = w(y);
@@ -1017,8 +1030,8 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
       const int first = static_cast<int>(sh.bracket[0]), last = static_cast<int>(sh.bracket[1]);
       // the bracket in scores, a little wider than the bins
       const float slack = 4e-7f * (fabsf(m) + static_cast<float>(last + 1) / per_unit);
-      const float high = m - static_cast<float>(first) / per_unit + slack;
-      const float low = m - static_cast<float>(last + 1) / per_unit - slack;
+      high = m - static_cast<float>(first) / per_unit + slack;
+      low = fmaxf(kLowest, m - static_cast<float>(last + 1) / per_unit - slack);
       u64 sum = 0;
       int over = 0;
       each_from(low, high,
@@ -1042,7 +1055,10 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
         const int n = static_cast<int>(sh.list_n);
         u64 above;
         before_warp(&above);
-        if (tid == 0) sh.state = 0;
+        if (tid == 0) {
+          sh.state = 0;
+          sh.edge = above;  // for the way by digits
+        }
         __syncthreads();
         if (n > 0 && n <= kList && above < target) {
           for (int i = tid; i < n; i += kThreads)
@@ -1081,10 +1097,11 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
         }
       }
       cluster.sync();
-      if (sh.state) edge = sh.edge;
       summed = sh.state == 2;
+      // more columns in the bracket than the list holds: they alone are gone through by digits
+      edge = sh.state ? sh.edge : reach(in, target, sh.edge, low, high, w);
     }
-    if (!binned || sh.state == 0) edge = reach(in, target, [&](float y) { return w(y); });
+    if (!binned || !edge) edge = reach(in, target, 0, kLowest, none, w);
   }
   if (o.mp_key > element_key(edge)) edge = element(o.mp_key, ~0u);
   auto kept_weight = [&](float y, int col) {
@@ -1157,18 +1174,9 @@ cudaError_t sample(const SampleParams& p, cudaStream_t stream) {
   static std::atomic<uint64_t> done[2];
   const cudaError_t e = allow_smem(kernel, 227 * 1024, done[one_pass]);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.rows * nb));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kFixed + static_cast<size_t>(resident) * 16;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(nb);
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p, frac_bits(p.cols), block_chunks, resident);
+  const LaunchShape shape{static_cast<unsigned>(p.rows * nb), kThreads,
+                          kFixed + static_cast<size_t>(resident) * 16, static_cast<unsigned>(nb)};
+  return launch(kernel, shape, stream, p, frac_bits(p.cols), block_chunks, resident);
 }
 
 }  // namespace

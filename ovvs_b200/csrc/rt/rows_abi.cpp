@@ -41,7 +41,11 @@ ovvsStatus launched(Resources& r, F&& launch) {
   try {
     DeviceScope scope;
     OVVS_TRY(scope.enter(r));
-    OVVS_TRY_CUDA(launch());
+    const cudaError_t e = launch();
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();  // a refused launch is reported once, by this call
+      return ovvs::rt::status_of(e);
+    }
     r.last_device = OVVS_DEVICE_GPU;
     return OVVS_STATUS_SUCCESS;
   } catch (...) {
