@@ -254,35 +254,45 @@ __device__ void sort_list(u64* a, int n) {
   __syncthreads();
 }
 
-// One warp: a bound that at least k of n <= 32 * kPer keys reach, and, where the keys allow it,
-// not many more; the key of the type's lowest value, which every score reaches, when fewer than
-// k do.
+// One warp: a bound that at least k of n keys reach, and, where the keys allow it, no more than
+// slack others; the key of the type's lowest value, which every score reaches, when fewer than k
+// are not 0. The keys, at most 32 * kPer, are held in registers, or for kPer = 0 read every time.
 template <int kPer>
-__device__ uint32_t kth_bound(const uint32_t* key, int n, int k) {
+__device__ uint32_t kth_bound(const uint32_t* key, int n, int k, int slack) {
   const int lane = threadIdx.x & 31;
-  uint32_t own[kPer], hi = 0, least = ~0u;
-  int valid = 0;
+  uint32_t own[kPer ? kPer : 1];
+  if constexpr (kPer != 0) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    own[i] = i * 32 + lane < n ? key[i * 32 + lane] : 0;
-    hi = max(hi, own[i]);
-    if (own[i]) {
-      least = min(least, own[i]);
+    for (int i = 0; i < kPer; ++i) own[i] = i * 32 + lane < n ? key[i * 32 + lane] : 0;
+  }
+  auto each = [&](auto&& f) {
+    if constexpr (kPer != 0) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) f(own[i]);
+    } else {
+      for (int i = lane; i < n; i += 32) f(key[i]);
+    }
+  };
+  uint32_t hi = 0, least = ~0u;
+  int valid = 0;
+  each([&](uint32_t y) {
+    hi = max(hi, y);
+    if (y) {
+      least = min(least, y);
       ++valid;
     }
-  }
+  });
   if (static_cast<int>(__reduce_add_sync(~0u, valid)) < k) return sort_key(-3.402823466e38f);
   hi = __reduce_max_sync(~0u, hi);
   uint32_t lo = __reduce_min_sync(~0u, least);
   while (lo < hi) {
     const uint32_t mid = lo + (hi - lo + 1) / 2;
     int c = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) c += own[i] >= mid;
+    each([&](uint32_t y) { c += y >= mid; });
     c = __reduce_add_sync(~0u, c);
     if (c >= k) {
       lo = mid;
-      if (c <= k + (k >> 3)) break;
+      if (c <= k + slack) break;
     } else {
       hi = mid - 1;
     }
@@ -608,7 +618,7 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     maxima[kThreads + tid] = sort_key(second);
     __syncthreads();
     if (warp == 0) {
-      const uint32_t found = kth_bound<2 * kThreads / 32>(maxima, 2 * kThreads, o.k);
+      const uint32_t found = kth_bound<2 * kThreads / 32>(maxima, 2 * kThreads, o.k, o.k >> 5);
       if (lane == 0) sh.pick = found;
     }
     __syncthreads();
@@ -678,7 +688,7 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
   // The `heads` largest of each warp's threads' maxima, on every block.
   uint32_t* maxima = reinterpret_cast<uint32_t*>(sh.pre);
   const uint32_t own_key = sort_key(own);
-  const int heads = direct ? min(min(32, 1024 / (nb * kWarps)), 1 + 2 * o.k / (nb * kWarps)) : 1;
+  const int heads = greedy || o.k <= 0 ? 1 : min(32, 1 + 2 * min(o.k, 2048) / (nb * kWarps));
   cluster.barrier_wait(std::move(started));  // every block runs: its shared memory may be written
   {
     uint32_t left = own_key;
@@ -742,17 +752,19 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
   w.set(m, t, frac, sh.table);
   o.mp_key = min_p_key(m, t, mp);
 
-  if (direct) {
-    // The largest bound found by halving that at least k maxima reach; every maximum is a score,
-    // so at least k scores reach it too.
+  float bound = -3.402823466e38f;
+  if (o.k > 0) {
+    // A bound that at least k maxima reach, found by halving; every maximum is a score, so at
+    // least k scores reach it too.
     if (warp == 0) {
-      const uint32_t found = num_maxima <= 128 ? kth_bound<4>(maxima, num_maxima, o.k)
-                                               : kth_bound<32>(maxima, num_maxima, o.k);
+      const uint32_t found = num_maxima <= 128 ? kth_bound<4>(maxima, num_maxima, o.k, o.k >> 3)
+                                               : kth_bound<0>(maxima, num_maxima, o.k, o.k >> 4);
       if (lane == 0) sh.pick = found;
     }
     __syncthreads();
-    const uint32_t lo = sh.pick;
-    const float bound = keys::order_value(lo);
+    bound = keys::order_value(sh.pick);
+  }
+  if (direct) {
     for (int c = c0 + lane; c < c1; c += 32) {
       const uint4 v = chunk_at(c);
       if (!(C::largest(v) >= bound)) continue;
@@ -834,9 +846,10 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     if (lane < nb) cluster.map_shared_rank(&sh, lane)->tot[rank * kWarps + warp] = s;
     cluster.sync();
   };
-  // The column of this warp's range at which before + the running sum passes target.
-  auto walk = [&](u64 before, u64 target, auto&& value, auto&& then) {
-    for (int c = c0; c < c1; c += 32) {
+  // then(column, value, i) for the column of this warp's range at which before + the running sum
+  // of value passes lane i's target, for every lane i of todo.
+  auto walk = [&](u64 before, u64 target, unsigned todo, auto&& value, auto&& then) {
+    for (int c = c0; c < c1 && todo; c += 32) {
       float y[C::kN];
       u64 v[C::kN], sum = 0;
       C::unpack(c + lane < c1 ? chunk_at(c + lane) : C::masked(), y);
@@ -852,23 +865,28 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
         const u64 z = __shfl_up_sync(~0u, s, i);
         if (lane >= i) s += z;
       }
-      const unsigned hit = __ballot_sync(~0u, before + s > target);
-      if (hit) {
-        if (lane == __ffs(hit) - 1) {
-          u64 run = before + s - sum;
+      s += before;
+      before = __shfl_sync(~0u, s, 31);
+      unsigned here = __ballot_sync(~0u, target < before) & todo;
+      todo &= ~here;
+      while (here) {
+        const int i = __ffs(here) - 1;
+        here &= here - 1;
+        const u64 t = __shfl_sync(~0u, target, i);
+        const unsigned passed = __ballot_sync(~0u, s > t);
+        if (lane == __ffs(passed) - 1) {
+          u64 run = s - sum;
           bool done = false;
 #pragma unroll
           for (int e = 0; e < C::kN; ++e) {
             run += v[e];
-            if (!done && run > target) {
-              then(col + e, v[e]);
+            if (!done && run > t) {
+              then(col + e, v[e], i);
               done = true;
             }
           }
         }
-        return;
       }
-      before += __shfl_sync(~0u, s, 31);
     }
   };
   auto before_warp = [&](u64* z) {
@@ -879,24 +897,26 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     return warp_reduce((lane < me ? a : 0) + (32 + lane < me ? b : 0), Add());
   };
   // Edge of the shortest prefix, among the columns up to `in`, whose sum of value(x) reaches
-  // target, where the scores from `high` on sum to `above` and it ends among those below from
-  // `low` on (0 if it does not): the score one 8-bit digit at a time, then the column among those
-  // that share it.
-  auto reach = [&](u64 in, u64 target, u64 above, float low, float high, auto&& value) -> u64 {
+  // target, where the scores whose key is above `khi` sum to `above` and it ends among those from
+  // `klo` to there (0 if it does not): the range of keys in 256 parts, then the part where it
+  // ends, until that is one score; then the column among those that hold it.
+  auto reach = [&](u64 in, u64 target, u64 above, uint32_t klo, uint32_t khi, auto&& value) -> u64 {
     u64* hist = sh.wts;
-    uint32_t prefix = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
+    for (bool one = false; !one;) {
+      const uint32_t span = khi - klo;
+      const int shift = span < 256 ? 0 : 24 - __clz(span);
+      one = shift == 0;
       cluster.sync();
       hist[tid] = 0;
       __syncthreads();
-      const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
-      uint32_t at = 0;  // equal scores in a row are added up before they go to their bin
+      const float low = keys::order_value(klo), high = keys::order_value(khi);
+      uint32_t at = 0;  // equal parts in a row are added up before they go to the histogram
       u64 sum = 0;
       each([&](float y, int col) {
-        if (!(y >= low) || y >= high) return;
+        if (!(y >= low) || !(y <= high)) return;
         const uint32_t k = sort_key(y);
-        if ((k & mask) != prefix || element(k, col) < in) return;
-        const uint32_t bin = k >> shift & 255;
+        if (k < klo || k > khi || element(k, col) < in) return;
+        const uint32_t bin = (k - klo) >> shift;
         if (bin != at && sum) {
           atomicAdd(&hist[at], sum);
           sum = 0;
@@ -915,29 +935,31 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
         sh.above = before;
       }
       __syncthreads();
-      prefix |= sh.pick << shift;
+      klo += sh.pick << shift;
+      const uint32_t rest = (1u << shift) - 1;
+      khi = khi - klo > rest ? klo + rest : khi;
       above = sh.above;
     }
-    const u64 v = value(keys::order_value(prefix));
+    const u64 v = value(keys::order_value(klo));
     const u64 ties = (target - above + v - 1) / v;
     auto tie = [&](float y, int col) {
       const uint32_t k = sort_key(y);
-      return u64{k == prefix && element(k, col) >= in};
+      return u64{k == klo && element(k, col) >= in};
     };
     u64 own_ties = 0, all;
     each([&](float y, int col) { own_ties += tie(y, col); });
     share_totals(own_ties);
     const u64 before = before_warp(&all);
     if (ties - 1 >= before && ties - 1 < before + sh.tot[rank * kWarps + warp])
-      walk(before, ties - 1, tie, [&](int col, u64) {
+      walk(before, ties - 1, 1, tie, [&](int col, u64, int) {
         for (int b = 0; b < nb; ++b) cluster.map_shared_rank(&sh, b)->found = col;
       });
     cluster.sync();
-    return element(prefix, static_cast<uint32_t>(sh.found));
+    return element(klo, static_cast<uint32_t>(sh.found));
   };
 
   constexpr float kLowest = -3.402823466e38f;
-  const float none = __int_as_float(0x7fffffff);  // no score reaches a NaN
+  const uint32_t lowest_key = sort_key(kLowest);
   const u64 everything = element(1, ~0u);  // every column that is not masked
   u64 edge = everything;
   if (o.k > 0) {
@@ -945,7 +967,8 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     each([&](float y, int) { n += y > -INFINITY; });
     n = cluster_sum(n);
     if (static_cast<u64>(o.k) < n)
-      edge = reach(edge, static_cast<u64>(o.k), 0, kLowest, none, [](float) { return u64{1}; });
+      edge = reach(edge, static_cast<u64>(o.k), 0, sort_key(bound), best,
+                   [](float) { return u64{1}; });
   }
   bool summed = false;  // tot holds the kept weights
   if (o.tp < 1.f) {
@@ -966,7 +989,7 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     __syncthreads();
     const float bins_f = binned ? static_cast<float>(kBins) : 0.f;
     const float unit_per_bin = 1.f / bins_per_unit;
-    float low = kLowest, high = none;
+    float low = kLowest, high = kLowest;
     u64 z = 0;
     auto weigh = [&](float y, bool in) {
       const u64 own = w(y);
@@ -1099,9 +1122,11 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
       cluster.sync();
       summed = sh.state == 2;
       // more columns in the bracket than the list holds: they alone are gone through by digits
-      edge = sh.state ? sh.edge : reach(in, target, sh.edge, low, high, w);
+      edge = sh.state ? sh.edge
+                      : reach(in, target, sh.edge, sort_key(low),
+                              max(sort_key(low), sort_key(high) - 1), w);
     }
-    if (!binned || !edge) edge = reach(in, target, 0, kLowest, none, w);
+    if (!binned || !edge) edge = reach(in, target, 0, lowest_key, best, w);
   }
   if (o.mp_key > element_key(edge)) edge = element(o.mp_key, ~0u);
   auto kept_weight = [&](float y, int col) {
@@ -1137,17 +1162,14 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
   for (int64_t d0 = 0; d0 < p.draws; d0 += 32) {
     const int64_t d = d0 + lane;
     const u64 target = d < p.draws ? draw_target(p.uniforms[row * p.draws + d], z) : 0;
-    unsigned todo = __ballot_sync(~0u, d < p.draws && target >= before && target - before < mine);
-    while (todo) {
-      const int i = __ffs(todo) - 1;
-      todo &= todo - 1;
-      walk(before, __shfl_sync(~0u, target, i), kept_weight, [&](int col, u64 v) {
-        p.ids[row * p.draws + d0 + i] = col;
-        if (p.probs)
-          p.probs[row * p.draws + d0 + i] =
-              static_cast<float>(static_cast<double>(v) / static_cast<double>(z));
-      });
-    }
+    const unsigned todo =
+        __ballot_sync(~0u, d < p.draws && target >= before && target - before < mine);
+    walk(before, target, todo, kept_weight, [&](int col, u64 v, int i) {
+      p.ids[row * p.draws + d0 + i] = col;
+      if (p.probs)
+        p.probs[row * p.draws + d0 + i] =
+            static_cast<float>(static_cast<double>(v) / static_cast<double>(z));
+    });
   }
 }
 
