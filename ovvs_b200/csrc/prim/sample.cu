@@ -82,7 +82,7 @@ struct Weigher {
   float cut;       // scores below it weigh 0
   bool top_inf;    // m is +inf: the columns that hold it weigh 1, the others 0
   int frac;
-  const double* table;
+  const double* table;  // 2^(i / 16 + frac)
 
   __device__ __forceinline__ void set(float max, float t, int frac_bits, const double* tab) {
     frac = frac_bits;
@@ -93,9 +93,8 @@ struct Weigher {
     const double low = m - static_cast<double>(t) * 0.6931471805599453 * (frac + 1);
     cut = fmaxf(__double2float_ru(low), -3.402823466e38f);
   }
-  // Without a branch, so that several weights are under way at once.
-  __device__ __forceinline__ u64 operator()(float x) const {
-    if (top_inf) x = x == INFINITY ? 0.f : -INFINITY;
+  // For x >= cut where m is finite. Without a branch, so that several are under way at once.
+  __device__ __forceinline__ u64 plain(float x) const {
     const double magic = 6755399441055744.0;  // 1.5 * 2^52
     const double d = static_cast<double>(x) - m;
     const double r = fma(d, rate, magic);
@@ -106,11 +105,14 @@ struct Weigher {
     p = fma(f, p, 0.043321698760160544);
     p = fma(f, p, 1.0);
     const double s = table[n & 15];
-    const double scaled = __hiloint2double(__double2hiint(s) + (frac + (n >> 4)) * (1 << 20),
+    const double scaled = __hiloint2double(__double2hiint(s) + (n & ~15) * (1 << 16),
                                            __double2loint(s));
     const double w = fma(p, scaled, 4503599627370496.0);
-    const u64 bits = static_cast<u64>(__double_as_longlong(w)) & ((u64{1} << 52) - 1);
-    return x >= cut ? bits : 0;
+    return static_cast<u64>(__double_as_longlong(w)) & ((u64{1} << 52) - 1);
+  }
+  __device__ __forceinline__ u64 operator()(float x) const {
+    if (top_inf) return x == INFINITY ? u64{1} << frac : 0;
+    return x >= cut ? plain(x) : 0;
   }
 };
 
@@ -132,14 +134,52 @@ struct Chunk {
   static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[kN]);
   // Largest of the chunk's scores that are not NaN; -inf without one.
   static __device__ __forceinline__ float largest(const uint4& v) {
-    float x[kN];
-    unpack(v, x);
-    float m = -INFINITY;
+    float m;
+    if constexpr (sizeof(T) == 4) {
+      m = fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)),
+                fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+    } else {
+      const Pair p = __hmax2(__hmax2(pair(v.x), pair(v.y)), __hmax2(pair(v.z), pair(v.w)));
+      m = score_f32(__hmax(p.x, p.y));
+    }
+    return fmaxf(m, -INFINITY);
+  }
+  // Marks of the scores that reach a bound (kGroup chunks make a word): where bit b of it stands.
+  using Pair = typename std::conditional<std::is_same<T, __half>::value, __half2,
+                                         __nv_bfloat162>::type;
+  using Bound = typename std::conditional<sizeof(T) == 4, float, Pair>::type;
+  static constexpr int kGroup = 32 / kN;
+  static __device__ __forceinline__ Pair pair(uint32_t w) {
+    return *reinterpret_cast<const Pair*>(&w);
+  }
+  static __device__ __forceinline__ Bound bound(float x);  // the first value that is not below x
+  static __device__ __forceinline__ uint32_t mark(const uint4& v, Bound b, int chunk) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t bits = 0;
 #pragma unroll
-    for (int e = 0; e < kN; ++e) m = fmaxf(m, x[e]);
-    return m;
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4)
+        bits |= __uint_as_float(w[i]) >= b ? 1u << (chunk * 4 + i) : 0u;
+      else
+        bits |= __hge2_mask(pair(w[i]), b) & 0x00010001u << (chunk * 4 + i);
+    }
+    return bits;
+  }
+  static __device__ __forceinline__ int chunk_of(int bit) { return (bit & (4 * kGroup - 1)) >> 2; }
+  static __device__ __forceinline__ int cell_of(int bit) {
+    return sizeof(T) == 4 ? bit & 3 : (bit & 3) * 2 + (bit >> 4);
   }
 };
+template <>
+__device__ __forceinline__ float Chunk<float>::bound(float x) { return x; }
+template <>
+__device__ __forceinline__ __half2 Chunk<__half>::bound(float x) {
+  return __half2half2(__float2half_ru(x));
+}
+template <>
+__device__ __forceinline__ __nv_bfloat162 Chunk<__nv_bfloat16>::bound(float x) {
+  return __bfloat162bfloat162(__float2bfloat16_ru(x));
+}
 template <>
 __device__ __forceinline__ void Chunk<float>::unpack(const uint4& v, float (&x)[4]) {
   x[0] = __uint_as_float(v.x);
@@ -584,7 +624,7 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
   const float mp = p.min_p ? p.min_p[row] : 0.f;
   const bool greedy = !(t > 0.f);
 
-  if (tid < 16) sh.table[tid] = kSixteenths[tid];
+  if (tid < 16) sh.table[tid] = ldexp(kSixteenths[tid], frac);
   if (tid == 0) {
     sh.list_n = 0;
     sh.staged = 0;
@@ -799,34 +839,36 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
       for (int e = 0; e < C::kN; ++e) f(y[e], col + e);
     }
   };
-  // f(score, column) for the scores from `high` on, g for those below it from `low` on. Each lane
-  // marks them among 32 of its scores first and then takes its marked ones, so that a warp does
-  // not go through the motions of f on every score for the few that need it.
-  auto each_from = [&](float low, float high, auto&& f, auto&& g) {
-    constexpr int kGroup = 32 / C::kN;
-    low = fmaxf(low, -3.402823466e38f);  // -inf stands where there is no column
-    high = fmaxf(high, low);
-    for (int c = c0 + lane; c < c1; c += 32 * kGroup) {
-      uint32_t above = 0, within = 0;
+  // Sum and number of the weights from `high` on, and rare(score, column) for the scores below it
+  // from `low` on. Each lane marks them among 32 of its scores first and then takes its marked
+  // ones, two at a time, so that a warp does not weigh every score for the few that need it.
+  const bool all_held = block_chunks <= resident;
+  auto sum_from = [&](float low, float high, u64* sum, int* number, auto&& rare) {
+    const auto bound = C::bound(fmaxf(low, -3.402823466e38f));  // -inf: there is no column
+    high = fmaxf(high, w.cut);
+    for (int c = c0 + lane; c < c1; c += 32 * C::kGroup) {
+      uint32_t marked = 0;
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) {
-        float y[C::kN];
-        C::unpack(c + i * 32 < c1 ? chunk_at(c + i * 32) : C::masked(), y);
-#pragma unroll
-        for (int e = 0; e < C::kN; ++e) {
-          above |= y[e] >= high ? 1u << (i * C::kN + e) : 0u;
-          within |= y[e] >= low ? 1u << (i * C::kN + e) : 0u;
-        }
-      }
-      within &= ~above;
-      auto take = [&](uint32_t& bits, auto&& h) {
-        const int bit = __ffs(bits) - 1;
-        bits &= bits - 1;
-        const int at = c + bit / C::kN * 32, e = bit % C::kN, col = first_col(at) + e;
-        h(score_f32(at < resident ? reinterpret_cast<const T*>(held + at)[e] : x[col]), col);
+      for (int i = 0; i < C::kGroup; ++i)
+        marked |= C::mark(c + i * 32 < c1 ? chunk_at(c + i * 32) : C::masked(), bound, i);
+      auto score_at = [&](int bit) {
+        const int at = c + C::chunk_of(bit) * 32, e = C::cell_of(bit);
+        if (all_held || at < resident) return score_f32(reinterpret_cast<const T*>(held + at)[e]);
+        return score_f32(x[first_col(at) + e]);
       };
-      while (within) take(within, g);
-      while (above) take(above, f);
+      while (marked) {
+        const int b0 = __ffs(marked) - 1;
+        marked &= marked - 1;
+        const int b1 = marked ? __ffs(marked) - 1 : -1;
+        marked &= marked - 1;
+        const float y0 = score_at(b0), y1 = b1 >= 0 ? score_at(b1) : -INFINITY;
+        const u64 v0 = w.plain(y0), v1 = w.plain(y1);
+        const bool in0 = y0 >= high, in1 = y1 >= high;
+        *sum += (in0 ? v0 : 0) + (in1 ? v1 : 0);
+        *number += in0 + in1;
+        if (!in0) rare(y0, first_col(c + C::chunk_of(b0) * 32) + C::cell_of(b0));
+        if (!in1 && b1 >= 0) rare(y1, first_col(c + C::chunk_of(b1) * 32) + C::cell_of(b1));
+      }
     }
   };
   int turn = 0;
@@ -974,7 +1016,6 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
   if (o.tp < 1.f) {
     const bool limited = edge != everything;
     const u64 in = edge;
-    auto inside = [&](float y, int col) { return !limited || element(sort_key(y), col) >= in; };
     // Bins of (m - x) / T. The edge's weight is at least (1 - p) / cols of the largest, so they
     // reach that far and no further: 100 to 200 a unit. A bin sums weights relative to its upper
     // end, in 1 / unit, from a second-order series: good to half a unit and 1e-6.
@@ -991,17 +1032,21 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     const float unit_per_bin = 1.f / bins_per_unit;
     float low = kLowest, high = kLowest;
     u64 z = 0;
+    // unit * exp(-g * unit_per_bin) to the second order
+    const float slope = -unit * unit_per_bin, bend = 0.5f * unit * unit_per_bin * unit_per_bin;
     auto weigh = [&](float y, bool in) {
-      const u64 own = w(y);
-      z += in ? own : 0;
+      const u64 own = w.plain(y);
       // the nearest bin below, and how far into it, without a conversion
       const float v = (m - y) * per_unit, vb = __fadd_rz(v, 8388608.f);
-      const float f = (v - (vb - 8388608.f)) * unit_per_bin;
-      const float q = fmaf(unit, 1.f - f * (1.f - 0.5f * f), 8388608.f);
+      const float g = v - (vb - 8388608.f);
+      const float q = fmaf(g, fmaf(g, bend, slope), unit + 8388608.f);
+      z += in && y >= w.cut ? own : 0;
       if (v < bins_f && in)
         atomicAdd(&hist[__float_as_uint(vb) & 0x7fffffu], __float_as_uint(q) - 0x4b000000u);
     };
-    if (limited)
+    if (w.top_inf)
+      each([&](float y, int col) { z += element(sort_key(y), col) >= in ? w(y) : 0; });
+    else if (limited)
       each([&](float y, int col) { weigh(y, element(sort_key(y), col) >= in); });
     else
       each([&](float y, int) { weigh(y, true); });
@@ -1057,15 +1102,19 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
       low = fmaxf(kLowest, m - static_cast<float>(last + 1) / per_unit - slack);
       u64 sum = 0;
       int over = 0;
-      each_from(low, high,
-                [&](float y, int col) {
-                  if (!inside(y, col)) return;
-                  sum += w(y);
-                  ++over;
-                },
-                [&](float y, int col) {
-                  if (inside(y, col)) stage(y, col);
-                });
+      if (limited) {
+        each([&](float y, int col) {
+          if (!(y >= low) || element(sort_key(y), col) < in) return;
+          if (y >= high) {
+            sum += w(y);
+            ++over;
+          } else {
+            stage(y, col);
+          }
+        });
+      } else {
+        sum_from(low, high, &sum, &over, stage);
+      }
       hand_over();
       sum = warp_reduce(sum, Add());
       over = __reduce_add_sync(~0u, over);
@@ -1133,26 +1182,32 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     return element(sort_key(y), col) >= edge ? w(y) : u64{0};
   };
   if (!summed) {
-    u64 sum = 0, n = 0;
+    u64 sum = 0;
+    int n = 0;
     if (edge == everything) {
       each([&](float y, int) {
         sum += w(y);
         n += y > -INFINITY;
       });
     } else {
-      auto take = [&](float y, int) {
+      const float last = keys::order_value(element_key(edge));
+      auto take = [&](float y, int col) {
+        if (y == last && static_cast<uint32_t>(col) > element_col(edge)) return;
         sum += w(y);
         ++n;
       };
-      const float last = keys::order_value(element_key(edge));
-      each_from(last, keys::order_value(element_key(edge) + 1), take, [&](float y, int col) {
-        if (static_cast<uint32_t>(col) <= element_col(edge)) take(y, col);
-      });
+      if (w.top_inf) {
+        each([&](float y, int col) {
+          if (y >= last) take(y, col);
+        });
+      } else {
+        sum_from(last, keys::order_value(element_key(edge) + 1), &sum, &n, take);
+      }
     }
     share_totals(sum);
     if (p.kept) {
-      n = cluster_sum(n);
-      if (rank == 0 && tid == 0) p.kept[row] = static_cast<int>(n);
+      const u64 all = cluster_sum(static_cast<u64>(n));
+      if (rank == 0 && tid == 0) p.kept[row] = static_cast<int>(all);
     }
   } else if (rank == 0 && tid == 0 && p.kept) {
     p.kept[row] = sh.cnt;
@@ -1192,9 +1247,10 @@ cudaError_t sample(const SampleParams& p, cudaStream_t stream) {
   const int block_chunks = static_cast<int>((chunks + nb - 1) / nb);
   const int most = static_cast<int>(((one_pass ? 45 : 227) * 1024 - kFixed) / 16);
   const int resident = block_chunks < most ? block_chunks : most;
-  auto kernel = one_pass ? sample_kernel<T, 5> : sample_kernel<T, 4>;
-  static std::atomic<uint64_t> done[2];
-  const cudaError_t e = allow_smem(kernel, 227 * 1024, done[one_pass]);
+  const int way = one_pass ? 2 : p.rows * nb > 592;
+  auto kernel = way == 2 ? sample_kernel<T, 5> : way ? sample_kernel<T, 4> : sample_kernel<T, 3>;
+  static std::atomic<uint64_t> done[3];
+  const cudaError_t e = allow_smem(kernel, 227 * 1024, done[way]);
   if (e != cudaSuccess) return e;
   const LaunchShape shape{static_cast<unsigned>(p.rows * nb), kThreads,
                           kFixed + static_cast<size_t>(resident) * 16, static_cast<unsigned>(nb)};

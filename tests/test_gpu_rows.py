@@ -172,6 +172,38 @@ def test_sample_masked(dtype, gpu, torch):
         check_sample(torch, gpu, x, u, temperature=[0.0] * 10)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sample_masked_stretches(dtype, gpu, torch):
+    """Long stretches of NaN and of -inf, in batches of each size class; what stands between them
+    is little, or together in one place, or in order."""
+    for rows, cols in ((300, 9001), (5, 40003)):
+        x = logits(torch, rows, cols, dtype, 23)
+        x[::2, 100:cols - 3000] = float("nan")
+        x[1::2, :cols - 50] = -float("inf")
+        x[2::5] = x[2::5].sort(1).values
+        x[3::5] = x[3::5].sort(1, descending=True).values
+        u = uniforms(24, rows, 2)
+        check_sample(torch, gpu, x, u, top_k=[40] * rows)
+        check_sample(torch, gpu, x, u, top_k=[40] * rows, top_p=[0.8] * rows)
+        check_sample(torch, gpu, x, u, top_p=[0.95] * rows)
+
+
+def test_sample_batch_of_many_kinds(gpu, torch):
+    """One large batch whose rows take every way: greedy, small and large top-k, top-p alone,
+    nothing, ties, all masked."""
+    rows, cols = 320, 7001
+    x = logits(torch, rows, cols, "float32", 25)
+    x[5::16] = x[5::16].round()
+    x[6::16] = 0.0
+    x[7::16] = -float("inf")
+    i = np.arange(rows)
+    check_sample(torch, gpu, x, uniforms(26, rows, 3),
+                 temperature=np.where(i % 8 == 0, 0.0, 0.5 + i % 5 * 0.4),
+                 top_k=np.array([0, 1, 50, 447, 448, 449, 2500, cols])[i // 2 % 8],
+                 top_p=np.array([1.0, 0.9, 0.3, 1.0, 0.99])[i % 5],
+                 min_p=np.array([0.0, 0.0, 0.02])[i % 3])
+
+
 def test_sample_odd_settings(gpu, torch):
     """Settings outside their ranges mean what the header says."""
     inf, nan = float("inf"), float("nan")
