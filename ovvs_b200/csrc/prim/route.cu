@@ -471,23 +471,24 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
     __syncwarp();
   }
   if (!listed) {
-    for (int r = 0; r < wanted; ++r) {
-      const uint32_t big = lanes_max<kLanes>(best);
-      doubt = doubt || (r && big && near(previous, big));
-      previous = big;
-      if (r == k) break;
 #pragma unroll
-      for (int j = 0; j < kSlots; ++j) {
-        if (j * kLanes + sub == r && big) {
-          id[j] = static_cast<int>(kIds - (big & kIds));
-          at[j] = big;
+    for (int j = 0; j < kSlots + 1; ++j) {
+      if (j * kLanes >= wanted) break;
+      for (int r = j * kLanes; r < min((j + 1) * kLanes, wanted); ++r) {
+        const uint32_t big = lanes_max<kLanes>(best);
+        doubt = doubt || (r && big && near(previous, big));
+        previous = big;
+        if (r == k) break;
+        if (j < kSlots && sub == r - j * kLanes && big) {
+          id[j < kSlots ? j : 0] = static_cast<int>(kIds - (big & kIds));
+          at[j < kSlots ? j : 0] = big;
         }
-      }
-      best = 0;
+        best = 0;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        key[i] = key[i] == big ? 0 : key[i];
-        best = max(best, key[i]);
+        for (int i = 0; i < kPer; ++i) {
+          key[i] = key[i] == big ? 0 : key[i];
+          best = max(best, key[i]);
+        }
       }
     }
   }
@@ -600,37 +601,39 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
     }
   }
 
-  // weights
+  // weights; slots beyond k hold nothing
   float y[kSlots], top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < kSlots; ++j) {
+    if (j * kLanes >= k) break;
     y[j] = id[j] >= 0 ? score_f32(x[id[j]]) : -INFINITY;
     top = fmaxf(top, y[j]);
   }
-  float w[kSlots], total = 0.f;
+  float w[kSlots], total = 0.f, inv = 1.f;
   if (p.renormalize) {
     top = lanes_max<kLanes>(top);
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
+      if (j * kLanes >= k) break;
       w[j] = id[j] >= 0 ? relative_score(y[j], top, p.sigmoid) : 0.f;
       total += w[j];
     }
     total = lanes_sum<kLanes>(total);  // 0, or at least a half
-    const float inv = total > 0.f ? rcp_fast(total) : 0.f;
-#pragma unroll
-    for (int j = 0; j < kSlots; ++j) w[j] *= inv;
+    inv = total > 0.f ? rcp_fast(total) : 0.f;
   } else {
 #pragma unroll
-    for (int j = 0; j < kSlots; ++j) w[j] = score(y[j]);
+    for (int j = 0; j < kSlots; ++j) {
+      if (j * kLanes >= k) break;
+      w[j] = score(y[j]);
+    }
   }
   if (live && !plain) {
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
       const int r = j * kLanes + sub;
-      if (r < k) {
-        p.ids[t * k + r] = id[j];
-        p.weights[t * k + r] = w[j] * p.scale;
-      }
+      if (r >= k) break;
+      p.ids[t * k + r] = id[j];
+      p.weights[t * k + r] = w[j] * inv * p.scale;
     }
   }
   unsigned again = __ballot_sync(~0u, plain && live && sub == 0);
@@ -668,17 +671,21 @@ route_backward_kernel(RouteBackwardParams p, bool whole, bool whole_out, bool wh
   int* id_of = reinterpret_cast<int*>(own_of + 32);
   const bool dense = p.dscores || (!p.sigmoid && !p.renormalize);
 
-  // the chosen: slot j of lane s is number j * kLanes + s
+  // the chosen: slot j of lane s is number j * kLanes + s; slots beyond k hold nothing
   int id[kSlots];
   float y[kSlots], dw[kSlots], top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < kSlots; ++j) {
+    id[j] = -1;
+    y[j] = -INFINITY;
+    dw[j] = 0.f;
+    if (j * kLanes >= k) continue;
     const int r = j * kLanes + sub;
-    id[j] = r < k ? p.ids[t * k + r] : -1;
+    if (r < k) id[j] = p.ids[t * k + r];
     if (id[j] >= n) id[j] = -1;
-    y[j] = id[j] >= 0 ? masked(score_f32(x[id[j]])) : -INFINITY;
+    if (id[j] >= 0) y[j] = masked(score_f32(x[id[j]]));
     if (!(y[j] > -INFINITY)) id[j] = -1;
-    dw[j] = id[j] >= 0 ? p.dweights[t * k + r] * p.scale : 0.f;
+    if (id[j] >= 0) dw[j] = p.dweights[t * k + r] * p.scale;
     top = fmaxf(top, y[j]);
   }
   float v[kPer], d[kPer], m = 0.f, inv_z = 0.f;
@@ -713,11 +720,14 @@ route_backward_kernel(RouteBackwardParams p, bool whole, bool whole_out, bool wh
   }
   // own: the chosen experts' part of the gradient; dot: what every softmax gradient subtracts
   float own[kSlots], dot = 0.f;
+#pragma unroll
+  for (int j = 0; j < kSlots; ++j) own[j] = 0.f;
   if (p.renormalize) {
     top = lanes_max<kLanes>(top);
     float total = 0.f, mean = 0.f;
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
+      if (j * kLanes >= k) break;
       own[j] = id[j] >= 0 ? relative_score(y[j], top, p.sigmoid) : 0.f;
       total += own[j];
     }
@@ -734,6 +744,7 @@ route_backward_kernel(RouteBackwardParams p, bool whole, bool whole_out, bool wh
   } else {
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
+      if (j * kLanes >= k) break;
       const float s = p.sigmoid ? sigmoid_fast(y[j])
                                 : (y[j] == m ? 1.f : exp_fast(y[j] - m)) * inv_z;
       own[j] = id[j] >= 0 ? s * dw[j] : 0.f;
@@ -742,8 +753,10 @@ route_backward_kernel(RouteBackwardParams p, bool whole, bool whole_out, bool wh
   }
   if (p.sigmoid) {
 #pragma unroll
-    for (int j = 0; j < kSlots; ++j)
+    for (int j = 0; j < kSlots; ++j) {
+      if (j * kLanes >= k) break;
       if (id[j] >= 0) own[j] *= sigmoid_fast(-y[j]);  // 1 - s
+    }
   } else if (dense) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) dot += v[i] * d[i];
