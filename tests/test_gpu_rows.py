@@ -763,6 +763,32 @@ def test_default_stream_is_the_resources_own(gpu, torch):
     assert gpu.last_device() == 3
 
 
+def test_outputs_that_are_left_out(gpu, torch):
+    """Without probabilities, kept counts and scores, the rest is the same."""
+    for rows, cols in ((3, 20001), (310, 3001)):
+        x = logits(torch, rows, cols, "bfloat16", 600)
+        u = torch.from_numpy(uniforms(601, rows, 2)).cuda()
+        for how in (dict(), dict(k=30), dict(p=0.9), dict(k=600, p=0.9), dict(t=0.0), dict(q=0.02),
+                    dict(p=0.9, q=0.02)):
+            put = lambda n, d: (torch.full((rows,), how[n], dtype=d, device="cuda")  # noqa: E731
+                                if n in how else None)
+            kw = dict(temperature=put("t", torch.float32), top_k=put("k", torch.int32),
+                      top_p=put("p", torch.float32), min_p=put("q", torch.float32), stream=0)
+            a = torch.empty(rows, 2, dtype=torch.int64, device="cuda")
+            b = torch.empty_like(a)
+            gpu.sample_rows(x, u, a, probs=torch.empty(rows, 2, device="cuda"),
+                            kept=torch.empty(rows, dtype=torch.int32, device="cuda"), **kw)
+            gpu.sample_rows(x, u, b, **kw)
+            assert torch.equal(a, b), how
+    x = logits(torch, 70, 256, "float32", 602)
+    ids = [torch.empty(70, 8, dtype=torch.int32, device="cuda") for _ in range(2)]
+    w = [torch.empty(70, 8, device="cuda") for _ in range(2)]
+    s = torch.empty(70, 256, device="cuda")
+    gpu.route_topk(x, ids[0], w[0], scores=s, stream=0)
+    gpu.route_topk(x, ids[1], w[1], stream=0)
+    assert torch.equal(ids[0], ids[1]) and torch.equal(w[0], w[1])
+
+
 def test_binding_refusals(gpu, torch):
     x = torch.zeros(4, 8, device="cuda")
     u = torch.zeros(4, device="cuda")
