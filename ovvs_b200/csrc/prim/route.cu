@@ -313,8 +313,16 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
   uint32_t key[kPer];
   if (need_scores) {
     float s[kPer];
+    if (p.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) s[i] = score(v[i]);
+      for (int i = 0; i < kPer; ++i) s[i] = v[i] > -INFINITY ? sigmoid_fast(v[i]) : 0.f;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const float e = v[i] == m ? 1.f : exp_fast(v[i] - m);
+        s[i] = v[i] > -INFINITY ? e * inv_z : 0.f;
+      }
+    }
     if (p.scores && live) store_cells<float, kPer>(p.scores + t * n, e0, n, whole_scores, s);
     if constexpr (kBias) {
       float b[kPer];
@@ -796,16 +804,15 @@ route_backward_kernel(RouteBackwardParams p, bool whole, bool whole_out, bool wh
     g[4 * i + 2] = c.z;
     g[4 * i + 3] = c.w;
   }
-  if (dense) {
+  if (dense && p.sigmoid) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      if (p.sigmoid) {
-        const float ex = exp_fast(-fabsf(v[i])), q = rcp_fast(1.f + ex);
-        if (v[i] > -INFINITY) g[i] += d[i] * ex * q * q;
-      } else {
-        g[i] += v[i] * (d[i] - dot);
-      }
+      const float ex = exp_fast(-fabsf(v[i])), q = rcp_fast(1.f + ex);
+      g[i] += v[i] > -INFINITY ? d[i] * ex * q * q : 0.f;
     }
+  } else if (dense) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) g[i] += v[i] * (d[i] - dot);
   }
   if (live) store_cells<T, kPer>(dx, e0, n, whole_out, g);
 }
