@@ -99,6 +99,7 @@ __device__ __forceinline__ void place_pairs(const int* ids, int64_t i0, int64_t 
     for (int j = 0; j < kAhead; ++j) ahead[j] = expert_of(ids, b + j * 32 + lane, i1, experts);
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
+      if (b + j * 32 >= i1) break;
       const int64_t i = b + j * 32 + lane;
       const int e = ahead[j];
       const unsigned same = same_expert(e, bits);
