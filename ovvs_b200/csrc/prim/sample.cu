@@ -631,35 +631,40 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     sh.first = ~0u;
   }
   auto started = cluster.barrier_arrive();
-  const bool direct = !greedy && o.k > 0 && o.k <= kDirectK;
+  const bool small = cols <= kList;  // the list holds the row (and one block takes it)
+  const bool direct = !greedy && (small || (o.k > 0 && o.k <= kDirectK));
   if (direct && nb == 1) {
     // One block for the row, nothing held. A look at every `skip`-th round of chunks, and the
     // last, gives a bound: the k-th of all threads' two best chunks. Then every column that
     // reaches it is listed, some k * skip of them; the rounds seen before come from L2.
     __syncthreads();
     uint32_t* maxima = reinterpret_cast<uint32_t*>(sh.pre);
-    const int skip = min(8, max(1, kWanted / o.k));
+    const int skip = small ? 1 : min(8, max(1, kWanted / o.k));
     const int rounds = (local + kRound * kThreads - 1) / (kRound * kThreads);
     uint4 v[kRound];
     auto load_round = [&](int r) {
       fetch_round(v, r * kRound * kThreads + tid, kThreads, local);
     };
-    float big = -INFINITY, second = -INFINITY;
-    for (int r = 0; r < rounds; r = r + 1 < rounds ? min(r + skip, rounds - 1) : rounds) {
-      load_round(r);
+    if (small) {
+      if (tid == 0) sh.pick = sort_key(-3.402823466e38f);
+    } else {
+      float big = -INFINITY, second = -INFINITY;
+      for (int r = 0; r < rounds; r = r + 1 < rounds ? min(r + skip, rounds - 1) : rounds) {
+        load_round(r);
 #pragma unroll
-      for (int i = 0; i < kRound; ++i) {
-        const float y = C::largest(v[i]);
-        second = fmaxf(second, fminf(big, y));
-        big = fmaxf(big, y);
+        for (int i = 0; i < kRound; ++i) {
+          const float y = C::largest(v[i]);
+          second = fmaxf(second, fminf(big, y));
+          big = fmaxf(big, y);
+        }
       }
-    }
-    maxima[tid] = sort_key(big);
-    maxima[kThreads + tid] = sort_key(second);
-    __syncthreads();
-    if (warp == 0) {
-      const uint32_t found = kth_bound<2 * kThreads / 32>(maxima, 2 * kThreads, o.k, o.k >> 5);
-      if (lane == 0) sh.pick = found;
+      maxima[tid] = sort_key(big);
+      maxima[kThreads + tid] = sort_key(second);
+      __syncthreads();
+      if (warp == 0) {
+        const uint32_t found = kth_bound<2 * kThreads / 32>(maxima, 2 * kThreads, o.k, o.k >> 5);
+        if (lane == 0) sh.pick = found;
+      }
     }
     __syncthreads();
     const float bound = keys::order_value(sh.pick);
@@ -693,7 +698,7 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     __syncthreads();
     unsigned listed = sh.list_n;
     if (fits && listed <= kList) {
-      if (listed > static_cast<unsigned>(o.k + o.k / 4)) {
+      if (o.k > 0 && o.k < kList && listed > static_cast<unsigned>(o.k + o.k / 4)) {
         const uint32_t lo = list_bound(sh, static_cast<int>(listed), o.k, sh.pick);
         listed = keep_listed(sh, static_cast<int>(listed), lo);
       }
@@ -1239,11 +1244,17 @@ cudaError_t sample(const SampleParams& p, cudaStream_t stream) {
   constexpr int kN = Chunk<T>::kN;
   constexpr size_t kFixed = (sizeof(Shared) + 15) / 16 * 16;
   const int64_t chunks = (p.cols + 2 * kN - 2) / kN;  // whatever the row's alignment
-  // A batch that fills the GPU with one block a row, and may have top-k rows, which that block
-  // then reads in one pass; otherwise up to a cluster a row, of blocks of 512 chunks or more.
+  // A batch of two rows an SM or more that may have top-k rows goes one block a row, which reads a
+  // top-k row in one pass (512 rows of 100,003 fp16, top-50: 32 us against 86 by clusters of 8;
+  // rows under top-p alone, which it reads again from L2, take 354 against 296). Otherwise a row
+  // gets a cluster: as many blocks as the SMs hold three of, of 512 chunks or more (16 rows of
+  // 32,000 bf16, top-p: 25 us by 8 blocks, 40 by 2), and beyond that as few as keep a block's
+  // part at 2048 chunks (400 such rows: 138 us by 8 blocks, 90 by 2, 112 by 1).
   const bool one_pass = p.top_k && p.rows >= 296;
   int nb = 1;
-  while (nb < kMaxCluster && chunks / nb > 512 && !one_pass) nb *= 2;
+  while (nb < kMaxCluster && !one_pass && chunks / nb > 512 &&
+         (p.rows * nb * 2 <= 444 || chunks / nb > 2048))
+    nb *= 2;
   const int block_chunks = static_cast<int>((chunks + nb - 1) / nb);
   const int most = static_cast<int>(((one_pass ? 45 : 227) * 1024 - kFixed) / 16);
   const int resident = block_chunks < most ? block_chunks : most;
