@@ -2,10 +2,13 @@
 // ranges of pairs and a row of counters each, so the place of a pair is its segment's start + the
 // pairs of its expert in earlier warps + those before it in its own warp.
 //
-// Up to kSmall pairs one block does it all (one launch: 4.8 us for 512 pairs of 256 experts).
-// Beyond that up to kMostBlocks blocks of kBlockPairs or more pairs work side by side, in four
-// launches with no workspace: the blocks' counts wait in `position` and the experts' in `offsets`,
-// whose own contents come last.
+// What bounds it: latency. Up to kSmall pairs one block does it all in one launch (256 experts:
+// 512 pairs 5.4 us, 4096 9; it would take 12 for 8192 and 18 for 16384). Beyond that up to
+// kMostBlocks blocks of kBlockPairs or more pairs work side by side, in four launches with no
+// workspace: the blocks' counts wait in `position` and the experts' in `offsets`, whose own
+// contents come last. Each launch is set up while the one before it runs. 4096 pairs would take
+// 11 us that way, 8192 to 131,072 take 12 to 14, 524,288 take 14.4 (17 without the early set-up).
+// The order's writes are scattered, a sector each: 6 MB move, 1 us at HBM's rate.
 #include "rows.cuh"
 
 namespace ovvs {
@@ -15,8 +18,8 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kSmall = 4096;
-constexpr int kBlockPairs = 4096;  // and multiples of it
-constexpr int kMostBlocks = 512;
+constexpr int kBlockPairs = 2048;  // and multiples of it
+constexpr int kMostBlocks = 148;   // one an SM
 static_assert(kBlockPairs >= kRouteMaxExperts, "position holds a count per block and expert");
 
 // The launches of a large plan follow one another closely: each says at once that the next may
@@ -99,7 +102,7 @@ __device__ __forceinline__ void place_pairs(const int* ids, int64_t i0, int64_t 
     for (int j = 0; j < kAhead; ++j) ahead[j] = expert_of(ids, b + j * 32 + lane, i1, experts);
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      if (b + j * 32 >= i1) break;
+      if (kPosition && b + j * 32 >= i1) break;  // a warp of a small plan has few
       const int64_t i = b + j * 32 + lane;
       const int e = ahead[j];
       const unsigned same = same_expert(e, bits);
@@ -121,6 +124,7 @@ route_plan_kernel(const int* ids, int64_t pairs, int experts, int align, int* of
                   int64_t capacity, int* position) {
   extern __shared__ int counts[];  // [kWarps][experts]
   __shared__ int buf[kWarps];
+  int* pad = counts + kWarps * experts;  // [2][experts]: where padding starts and ends
   const int tid = threadIdx.x, warp = tid >> 5;
   const int64_t span = ((pairs + kWarps - 1) / kWarps + 31) / 32 * 32;
   const int64_t i0 = warp * span, i1 = i0 + span < pairs ? i0 + span : pairs;
@@ -143,11 +147,14 @@ route_plan_kernel(const int* ids, int64_t pairs, int experts, int align, int* of
       counts[w * experts + tid] = next;
       next += c;
     }
-    for (int i = total; i < padded; ++i) order[first + i] = -1;
+    pad[tid] = first + total;
+    pad[experts + tid] = first + padded;
   }
   for (int64_t i = all + tid; i < capacity; i += kThreads) order[i] = -1;
   __syncthreads();
   place_pairs<true>(ids, i0, i1, experts, counts, order, position);
+  for (int x = warp; x < experts; x += kWarps)  // a warp an expert
+    for (int i = pad[x] + (tid & 31); i < pad[experts + x]; i += 32) order[i] = -1;
 }
 
 // Large plans, first: the pairs of each expert in every block of pairs, to table[expert][block].
@@ -178,7 +185,7 @@ plan_sum_kernel(int experts, int blocks, int* table, int* totals) {
   wait_for_last();
   if (e >= experts) return;
   int* row = table + e * blocks;
-  constexpr int kPer = kMostBlocks / 32;
+  constexpr int kPer = (kMostBlocks + 31) / 32;
   int c[kPer], run = 0;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) c[j] = j * 32 + lane < blocks ? row[j * 32 + lane] : 0;
@@ -230,8 +237,11 @@ plan_order_kernel(const int* ids, int64_t pairs, int64_t block_pairs, int expert
   }
   __syncthreads();
   place_pairs<false>(ids, i0, i1, experts, counts, order, nullptr);
-  for (int x = block; x < experts; x += blocks)
-    for (int i = pad[x] + tid; i < pad[experts + x]; i += kThreads) order[i] = -1;
+  // four warps an expert's padding, so that a tile of 128 rows takes one write
+  for (int x = block + tid / 128 * blocks; x < experts; x += blocks * (kThreads / 128)) {
+    const int end = pad[experts + x];
+    for (int i = pad[x] + tid % 128; i < end; i += 128) order[i] = -1;
+  }
   for (int64_t i = all + static_cast<int64_t>(block) * kThreads + tid; i < capacity;
        i += static_cast<int64_t>(blocks) * kThreads)
     order[i] = -1;
@@ -266,13 +276,13 @@ plan_position_kernel(const int* ids, int64_t pairs, int experts, int align, cons
 cudaError_t launch_route_plan(const int* ids, int64_t pairs, int experts, int align,
                               int* offsets, int* order, int64_t capacity, int* position,
                               cudaStream_t stream) {
-  const int smem = kWarps * experts * static_cast<int>(sizeof(int));
+  const size_t smem = static_cast<size_t>(kWarps + 2) * experts * sizeof(int);
   constexpr int kMost = (kWarps + 2) * kRouteMaxExperts * static_cast<int>(sizeof(int));
   if (pairs <= kSmall) {
     static std::atomic<uint64_t> done;
     const cudaError_t e = allow_smem(route_plan_kernel, kMost, done);
     if (e != cudaSuccess) return e;
-    return launch(route_plan_kernel, {1, kThreads, static_cast<size_t>(smem)}, stream, ids, pairs,
+    return launch(route_plan_kernel, {1, kThreads, smem}, stream, ids, pairs,
                   experts, align, offsets, order, capacity, position);
   }
   static std::atomic<uint64_t> done;
@@ -290,7 +300,10 @@ cudaError_t launch_route_plan(const int* ids, int64_t pairs, int experts, int al
   shape = {sum_blocks, kThreads, 0, 1, true};
   e = launch(plan_sum_kernel, shape, stream, experts, static_cast<int>(blocks), position, offsets);
   if (e != cudaSuccess) return e;
-  shape = {blocks, kThreads, smem + 2 * experts * sizeof(int), 1, true};
+  // more than half of an SM's shared memory: its blocks are set up early, and two on one SM beside
+  // idle ones would take longer (14.4 us for 524,288 pairs against 17.8)
+  constexpr size_t kAlone = 116 * 1024;
+  shape = {blocks, kThreads, smem > kAlone ? smem : kAlone, 1, true};
   e = launch(plan_order_kernel, shape, stream, ids, pairs, block_pairs, experts, align, position,
              offsets, order, capacity);
   if (e != cudaSuccess) return e;
