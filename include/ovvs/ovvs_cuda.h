@@ -128,9 +128,10 @@ OVVS_API ovvsStatus ovvsIvfFlatSearchDevice(ovvsResources_t res, ovvsIvfFlatInde
 
 /* The drawn and the trained counterparts of ovvsTopk, for scores that are already on the GPU: a
    search's scores, a router's or a language model's logits. All pointers are device pointers on
-   the Resources' device, aligned to their element. Each call checks its arguments, enqueues its
-   kernel on `stream` (NULL = the default stream) and returns; it uses no workspace and takes no
-   lock, so calls may run at once and may be captured into CUDA graphs. The caller's current
+   the Resources' device, aligned to their element; sizes have to be positive. Each call checks
+   its arguments (INVALID_ARGUMENT, or SHAPE_MISMATCH where a size is beyond a limit), enqueues
+   its kernels on `stream` (NULL = the default stream) and returns; it uses no workspace and takes
+   no lock, so calls may run at once and may be captured into CUDA graphs. The caller's current
    device is left as it was. Not in the reference.
 
    Order: larger scores first, equal ones (-0 equals +0) by lower column, as ovvsTopk with

@@ -60,7 +60,7 @@ constexpr int kRound = 8;       // chunks a thread has in flight where one block
 constexpr int kWanted = 520;    // columns it means to list
 constexpr int kNoted = 16;      // chunks a thread can note there
 constexpr int kBins = 2048;     // of the weight histogram
-static_assert(kBins * sizeof(float) == kList * sizeof(uint64_t), "the list holds the histogram");
+static_assert(kBins * sizeof(float) == kList * sizeof(uint64_t), "wts holds the histogram, pre its totals");
 
 using u64 = unsigned long long;
 
