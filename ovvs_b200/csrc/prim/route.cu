@@ -41,9 +41,16 @@ constexpr int kThreads = kWarps * 32;
 // reciprocal. A softmax by at most 49 * 2^-24: the same for its numerator, and its sum of up to
 // 1024 terms. Adding the bias rounds by up to 4 * 2^-24 and the code by half a unit: 1.1 units
 // for a sigmoid, 3.9 for a softmax (0.6 and 2 of the coarser units, and one that is cut off).
-// Codes of a pair no further apart than twice that, rounded up, are in doubt; of sums of two,
-// twice as far and two more.
+// Codes of a pair no further apart than twice that, rounded up, are in doubt.
 constexpr int kNearSigmoid = 3, kNearSoftmax = 9;
+
+// A group's sum of two is not made of codes, of which one that is cut off says nothing of the sum,
+// but of fp32 values s + b of any size. It is off by at most two scores' errors, half a step of
+// each part and of itself: 8.6 or 98 + 2 (|a| + |b|) in units of 2^-24; the bounds below leave room
+// for their own rounding. What stands has to be clear of what falls by both errors; sums beyond
+// fp32 are infinite, and in doubt among one another, as the bound stays finite.
+constexpr float kUnit = 1.f / (1 << 24);
+constexpr float kOffSigmoid = 9.f * kUnit, kOffSoftmax = 99.f * kUnit;
 
 __device__ __forceinline__ bool better(double a, int i, double b, int j) {
   return a > b || (a == b && i < j);
@@ -93,7 +100,12 @@ __device__ __forceinline__ float masked(float v) { return v > -INFINITY ? v : -I
 __device__ __forceinline__ uint32_t fixed_code(float c) {
   return __float_as_uint(fminf(fmaxf(c + 12.f, 8.000001f), 15.999999f)) & 0x7fffffu;
 }
-constexpr uint32_t kFixedZero = 4u << 20;  // fixed_code(0)
+
+// Order-preserving image of what is not a NaN; -0 comes before +0.
+__device__ __forceinline__ uint32_t image(float v) {
+  const int u = __float_as_int(v);
+  return static_cast<uint32_t>(u ^ (u >> 31 | static_cast<int>(0x80000000u)));
+}
 
 __device__ __forceinline__ float exp_fast(float x) {  // 2^-22 and the argument's rounding
   float y;
@@ -338,6 +350,7 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
         const float c = s[i] + b[i];
         const bool can = v[i] > -INFINITY && c > -INFINITY;
         key[i] = can ? fixed_code(c) >> kDrop << kIdBits | (kIds - (e0 + i)) : 0u;
+        v[i] = can ? c : -INFINITY;  // from here on
       }
     }
   }
@@ -357,6 +370,7 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
   if (p.groups > 1) {
     const int group = sub / group_lanes;
     uint32_t value;  // the group's, on its lanes, made unique by its number
+    float sum = 0.f, off = 0.f;
     if (!sums) {
       value = key[0];
 #pragma unroll
@@ -364,41 +378,30 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
       for (int o = 1; o < group_lanes; o <<= 1)
         value = max(value, __shfl_xor_sync(~0u, value, o));
     } else {
-      uint32_t a = 0, b = 0;  // the two best of the codes, or of the logits
-      float fa = -INFINITY, fb = -INFINITY;
+      // the group's two best s + b, or its two best logits, whose scores make the sum
+      float first = -INFINITY, second = -INFINITY;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        if constexpr (kBias) {
-          b = max(b, min(a, key[i]));
-          a = max(a, key[i]);
-        } else {
-          const float y = masked(v[i]);
-          fb = fmaxf(fb, fminf(fa, y));
-          fa = fmaxf(fa, y);
-        }
+        const float y = kBias ? v[i] : masked(v[i]);
+        second = fmaxf(second, fminf(first, y));
+        first = fmaxf(first, y);
       }
       for (int o = 1; o < group_lanes; o <<= 1) {
-        if constexpr (kBias) {
-          const uint32_t a2 = __shfl_xor_sync(~0u, a, o), b2 = __shfl_xor_sync(~0u, b, o);
-          b = max(min(a, a2), max(b, b2));
-          a = max(a, a2);
-        } else {
-          const float a2 = __shfl_xor_sync(~0u, fa, o), b2 = __shfl_xor_sync(~0u, fb, o);
-          fb = fmaxf(fminf(fa, a2), fmaxf(fb, b2));
-          fa = fmaxf(fa, a2);
-        }
+        const float a = __shfl_xor_sync(~0u, first, o), b = __shfl_xor_sync(~0u, second, o);
+        second = fmaxf(fminf(first, a), fmaxf(second, b));
+        first = fmaxf(first, a);
       }
-      // their sum in units of 2^-20, from 0 up
-      constexpr uint32_t kZero = kFixedZero >> kDrop;
+      const bool one = first > -INFINITY;
       if constexpr (kBias) {
-        value = (1u << 24) + (a >> kIdBits) - kZero + (b ? (b >> kIdBits) - kZero : 0);
-        if (!a) value = 0;
+        second = second > -INFINITY ? second : 0.f;
       } else {
-        value = (1u << 24) + fixed_code(score(fa)) - kFixedZero +
-                (fb > -INFINITY ? fixed_code(score(fb)) - kFixedZero : 0);
-        if (!(fa > -INFINITY)) value = 0;
+        first = score(first);
+        second = score(second);
       }
-      value = value ? value << 5 | (31 - group) : 0;
+      sum = first + second;
+      off = fminf(fmaf(4.f * kUnit, fabsf(first) + fabsf(second),
+                       p.sigmoid ? kOffSigmoid : kOffSoftmax), 3e38f);
+      value = one ? (image(sum) & ~31u) | (31 - group) : 0;
     }
     uint32_t left = value, last = 0;
     for (int i = 0; i < p.topk_groups; ++i) {
@@ -406,14 +409,14 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
       left = left == big ? 0 : left;
       last = big;
     }
-    const uint32_t fell = lanes_max<kLanes>(left);
-    if (last && fell) {
-      if (sums) {
-        const uint32_t far = 2 * (p.sigmoid ? kNearSigmoid : kNearSoftmax) + 2;
-        plain = (last >> 5) - (fell >> 5) <= far;
-      } else {
-        plain = near(last, fell);
-      }
+    if (!sums) {
+      const uint32_t fell = lanes_max<kLanes>(left);
+      plain = last && fell && near(last, fell);
+    } else {
+      // the highest that a group that fell may be, and the lowest that one that stands may be
+      const uint32_t high = lanes_max<kLanes>(left ? image(sum + off) : 0u);
+      const uint32_t low = ~lanes_max<kLanes>(left == value ? 0u : ~image(sum - off));
+      plain = high && low <= high;
     }
     if (left) {
 #pragma unroll

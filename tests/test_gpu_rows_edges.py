@@ -1,0 +1,64 @@
+"""Row operators on the GPU where a kernel's shortcut could show: biases of any size, ids at the
+ends of a packed key, gradients that are not finite, weights and scores held to the accuracy that
+is stated for them, places near 2^31."""
+
+import numpy as np
+import pytest
+
+from tests import rows_reference as ref
+from tests.test_gpu_rows import TYPES, check_route, logits, torch  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- routing: biases of any size ------------------------------------------------------------------
+
+def biases(experts, groups):
+    """name -> bias [experts]: what a router's balance bias may come to, and what blocks or forces
+    an expert."""
+    rng = np.random.default_rng(experts)
+    per = experts // groups
+    normal = lambda mean, std: rng.normal(mean, std, experts).astype(np.float32)  # noqa: E731
+    out = {"wide": normal(0, 2), "drifted": normal(6, 1), "off_centre": normal(2, 1),
+           "drifted_narrow": normal(6, 0.1), "far_below": normal(-40, 3)}
+    # one large value against a group of middling ones: their sums, not their parts, decide
+    one = np.zeros(experts, np.float32)
+    one[0] = 10.0
+    one[per:2 * per] = 3.0
+    out["one_of_ten"] = one
+    for v in (3.0, 5.0, 1e4, 3e38, np.inf):
+        for sign in (1, -1):
+            b = normal(0, 0.1)
+            b[rng.integers(0, experts, 3)] = sign * v
+            out[f"few_at_{sign * v:g}"] = b
+    alone = np.full(experts, -1e9, np.float32)  # every group but one expert disabled
+    alone[::per] = normal(0, 0.5)[::per]
+    out["one_left_a_group"] = alone
+    mixed = normal(0, 0.1)
+    mixed[::2] = -5.0
+    mixed[1::4] = -1e9
+    out["disabled_beside_low"] = mixed
+    return out
+
+
+@pytest.mark.parametrize("experts,groups,topk_groups,k", [
+    (64, 8, 1, 4), (64, 8, 3, 8), (128, 8, 4, 6), (256, 8, 4, 8), (256, 32, 9, 8), (512, 16, 5, 8),
+    (1024, 32, 7, 8), (160, 8, 3, 6)])
+def test_route_groups_with_any_bias(experts, groups, topk_groups, k, gpu, torch):  # noqa: F811
+    """A group's value is the sum of its two best s + b whatever the size of the biases."""
+    for i, (name, bias) in enumerate(biases(experts, groups).items()):
+        x = logits(torch, 70, experts, TYPES[i % 3], experts + i, 1.5)
+        x[0] = 0.0
+        x[1, ::3] = -float("inf")
+        for score in ("sigmoid", "softmax"):
+            for rule in ("top2", "max"):
+                check_route(torch, gpu, x, k, bias=bias, score=score, groups=groups,
+                            topk_groups=topk_groups, group_rule=rule, renormalize=i % 2 == 0)
+
+
+def test_route_any_bias_without_groups(gpu, torch):  # noqa: F811
+    for experts in (64, 128, 256, 1024):
+        for i, bias in enumerate(biases(experts, 8).values()):
+            x = logits(torch, 70, experts, TYPES[i % 3], experts + i, 1.5)
+            for score in ("sigmoid", "softmax"):
+                check_route(torch, gpu, x, 8, bias=bias, score=score)
