@@ -95,10 +95,11 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
 // -inf and NaN are masked.
 __device__ __forceinline__ float masked(float v) { return v > -INFINITY ? v : -INFINITY; }
 
-// c in units of 2^-20 above -4: c + 12 lies in [8, 16), where a float's last bit is one unit.
-// Never 0, which marks what cannot be chosen.
+// c in units of 2^-20 above -4: c + 12 lies in [8, 16), where a float's last bit is one unit. At
+// least 2, so that a code without its last bit is not 0 either: with the id 0 that would mark what
+// cannot be chosen.
 __device__ __forceinline__ uint32_t fixed_code(float c) {
-  return __float_as_uint(fminf(fmaxf(c + 12.f, 8.000001f), 15.999999f)) & 0x7fffffu;
+  return __float_as_uint(fminf(fmaxf(c + 12.f, 8.000002f), 15.999999f)) & 0x7fffffu;
 }
 
 // Order-preserving image of what is not a NaN; -0 comes before +0.

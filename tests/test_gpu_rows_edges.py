@@ -62,3 +62,22 @@ def test_route_any_bias_without_groups(gpu, torch):  # noqa: F811
             x = logits(torch, 70, experts, TYPES[i % 3], experts + i, 1.5)
             for score in ("sigmoid", "softmax"):
                 check_route(torch, gpu, x, 8, bias=bias, score=score)
+
+
+@pytest.mark.parametrize("experts", [8, 64, 255, 256, 257, 512, 1000, 1024])
+def test_route_last_expert_far_below(experts, gpu, torch):  # noqa: F811
+    """An expert that can be chosen is chosen, the last one and one of the lowest choice value
+    among them: -1 stands only where none is left."""
+    for last in (-5.0, -4.6, -1e9, -3e38):
+        bias = np.zeros(experts, np.float32)
+        bias[-1] = last
+        x = logits(torch, 4, experts, "float32", experts)
+        x[0, :-1] = -float("inf")
+        x[1, 2:-1] = -float("inf")
+        x[2, 1:] = -float("inf")
+        x[2, -1] = 0.5
+        for score in ("sigmoid", "softmax"):
+            for k in (1, 4, 8):
+                got = check_route(torch, gpu, x, k, bias=bias, score=score)
+                assert got[0][0, 0] == experts - 1
+                check_route(torch, gpu, x, k, bias=np.full(experts, last, np.float32), score=score)
