@@ -134,7 +134,7 @@ route_plan_kernel(const int* ids, int64_t pairs, int experts, int align, int* of
 #pragma unroll 8
     for (int w = 0; w < kWarps; ++w) total += counts[w * experts + tid];
   }
-  const int padded = (total + align - 1) / align * align;
+  const int padded = (total + (align - 1)) / align * align;
   int all;
   const int first = block_scan(padded, buf, &all);
   if (tid < experts) {
@@ -150,11 +150,15 @@ route_plan_kernel(const int* ids, int64_t pairs, int experts, int align, int* of
     pad[tid] = first + total;
     pad[experts + tid] = first + padded;
   }
-  for (int64_t i = all + tid; i < capacity; i += kThreads) order[i] = -1;
+  // places go up to 2^31 - 2, a thread's steps beyond
+  const uint32_t places = static_cast<uint32_t>(capacity);
+  for (uint32_t i = static_cast<uint32_t>(all) + tid; i < places; i += kThreads) order[i] = -1;
   __syncthreads();
   place_pairs<true>(ids, i0, i1, experts, counts, order, position);
-  for (int x = warp; x < experts; x += kWarps)  // a warp an expert
-    for (int i = pad[x] + (tid & 31); i < pad[experts + x]; i += 32) order[i] = -1;
+  for (int x = warp; x < experts; x += kWarps) {  // a warp an expert
+    const uint32_t end = pad[experts + x];
+    for (uint32_t i = static_cast<uint32_t>(pad[x]) + (tid & 31); i < end; i += 32) order[i] = -1;
+  }
 }
 
 // Large plans, first: the pairs of each expert in every block of pairs, to table[expert][block].
@@ -221,7 +225,7 @@ plan_order_kernel(const int* ids, int64_t pairs, int64_t block_pairs, int expert
   wait_for_last();
   const int total = tid < experts ? __ldcg(totals + tid) : 0;
   const int before = tid < experts ? __ldcg(table + tid * blocks + block) : 0;
-  const int padded = (total + align - 1) / align * align;
+  const int padded = (total + (align - 1)) / align * align;
   int all;
   const int first = block_scan(padded, buf, &all);
   if (tid < experts) {
@@ -239,8 +243,8 @@ plan_order_kernel(const int* ids, int64_t pairs, int64_t block_pairs, int expert
   place_pairs<false>(ids, i0, i1, experts, counts, order, nullptr);
   // four warps an expert's padding, so that a tile of 128 rows takes one write
   for (int x = block + tid / 128 * blocks; x < experts; x += blocks * (kThreads / 128)) {
-    const int end = pad[experts + x];
-    for (int i = pad[x] + tid % 128; i < end; i += 128) order[i] = -1;
+    const uint32_t end = pad[experts + x];
+    for (uint32_t i = static_cast<uint32_t>(pad[x]) + tid % 128; i < end; i += 128) order[i] = -1;
   }
   for (int64_t i = all + static_cast<int64_t>(block) * kThreads + tid; i < capacity;
        i += static_cast<int64_t>(blocks) * kThreads)
@@ -265,7 +269,7 @@ plan_position_kernel(const int* ids, int64_t pairs, int experts, int align, cons
   if (blockIdx.x == 0) {
     const int total = tid < experts ? offsets[tid] : 0;
     int all;
-    const int first = block_scan((total + align - 1) / align * align, buf, &all);
+    const int first = block_scan((total + (align - 1)) / align * align, buf, &all);
     if (tid < experts) offsets[tid] = first;
     if (tid == 0) offsets[experts] = all;
   }

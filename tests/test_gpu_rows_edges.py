@@ -81,3 +81,24 @@ def test_route_last_expert_far_below(experts, gpu, torch):  # noqa: F811
                 got = check_route(torch, gpu, x, k, bias=bias, score=score)
                 assert got[0][0, 0] == experts - 1
                 check_route(torch, gpu, x, k, bias=np.full(experts, last, np.float32), score=score)
+
+
+# ---- plan: places near 2^31 -------------------------------------------------------------------------
+
+def test_plan_padding_up_to_the_last_place(gpu, torch):  # noqa: F811
+    """Segments that end at place 2^31 - 1 or next to it: the padding is -1 to its end, in one
+    block's plan (a single pair) and in a large one (2^30 pairs)."""
+    for pairs, align in ((1, 2 ** 31 - 1), (2 ** 30, 2 ** 30 - 1)):
+        capacity = pairs + align - 1
+        ids = torch.zeros(pairs, dtype=torch.int32, device="cuda")
+        offsets = torch.empty(2, dtype=torch.int32, device="cuda")
+        order = torch.full((capacity,), 7, dtype=torch.int32, device="cuda")
+        position = torch.empty_like(ids)
+        gpu.route_plan(ids, 1, offsets, order, position, align=align, stream=0)
+        end = -(-pairs // align) * align
+        assert end == capacity and offsets.tolist() == [0, end]
+        assert torch.equal(order[:pairs], torch.arange(pairs, dtype=torch.int32, device="cuda"))
+        assert torch.equal(position, order[:pairs])
+        assert (order[pairs:] == -1).all()
+        del ids, order, position
+        torch.cuda.empty_cache()
