@@ -820,9 +820,9 @@ route_backward_kernel(RouteBackwardParams p, bool whole, bool whole_out, bool wh
       const float ex = exp_fast(-fabsf(v[i])), q = rcp_fast(1.f + ex);
       g[i] += v[i] > -INFINITY ? d[i] * ex * q * q : 0.f;
     }
-  } else if (dense) {
+  } else if (dense) {  // 0 where the score is 0, whatever dot is
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) g[i] += v[i] * (d[i] - dot);
+    for (int i = 0; i < kPer; ++i) g[i] += v[i] > 0.f ? v[i] * (d[i] - dot) : 0.f;
   }
   if (live) store_cells<T, kPer>(dx, e0, n, whole_out, g);
 }

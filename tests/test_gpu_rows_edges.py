@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from tests import rows_reference as ref
-from tests.test_gpu_rows import TYPES, check_route, logits, torch  # noqa: F401
+from tests.test_gpu_rows import TYPES, check_route, logits, run_backward, torch  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +102,32 @@ def test_plan_padding_up_to_the_last_place(gpu, torch):  # noqa: F811
         assert (order[pairs:] == -1).all()
         del ids, order, position
         torch.cuda.empty_cache()
+
+
+# ---- gradient: what is not finite ------------------------------------------------------------------
+
+@pytest.mark.parametrize("experts", [24, 64, 100, 256, 1000])
+def test_gradient_of_masked_stays_zero(experts, gpu, torch):  # noqa: F811
+    """A gradient that overflowed (inf or NaN at an expert that takes part) leaves masked experts
+    at 0: they have no part in the scores."""
+    for dtype in TYPES:
+        x = logits(torch, 9, experts, dtype, experts)
+        x[:, 1::4] = -float("inf")
+        x[:, 2::4] = float("nan")
+        masked = ~(x > -float("inf")).cpu().numpy()
+        xs = x.double().cpu().numpy()
+        for score in ("softmax", "sigmoid"):
+            for renormalize in (True, False):
+                ids = ref.route(xs, 4, score=score)[0]
+                for bad in (np.inf, -np.inf, np.nan):
+                    for where in ("weights", "scores"):
+                        dw = np.ones((9, 4), np.float32)
+                        ds = np.ones((9, experts), np.float32)
+                        if where == "weights":
+                            dw[:, 1] = bad
+                        else:
+                            ds[:, 0] = bad
+                        for dense in (True, False):
+                            got = run_backward(torch, gpu, x, ids, dw, ds if dense else None,
+                                               score=score, renormalize=renormalize, scale=1.0)
+                            assert (got[masked] == 0).all(), (score, renormalize, bad, where)
