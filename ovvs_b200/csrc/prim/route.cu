@@ -242,8 +242,8 @@ __global__ void __launch_bounds__(kThreads) route_plain_kernel(RouteParams p) {
 }
 
 // Loads or stores the kPer neighbours of a row from column e0 on; `whole` rows allow 16-byte
-// (or, for fewer bytes, one) accesses.
-template <class T, int kPer>
+// (or, for fewer bytes, one) accesses. kConst: nothing that the kernel writes may lie there.
+template <class T, int kPer, bool kConst = true>
 __device__ __forceinline__ void load_cells(const T* row, int e0, int n, bool whole,
                                            float (&v)[kPer], float other) {
   constexpr int kBytes = kPer * sizeof(T);
@@ -252,8 +252,10 @@ __device__ __forceinline__ void load_cells(const T* row, int e0, int n, bool who
       T raw[kPer];
       if constexpr (kBytes >= 16) {
 #pragma unroll
-        for (int i = 0; i < kBytes / 16; ++i)
-          reinterpret_cast<uint4*>(raw)[i] = __ldg(reinterpret_cast<const uint4*>(row + e0) + i);
+        for (int i = 0; i < kBytes / 16; ++i) {
+          const uint4* from = reinterpret_cast<const uint4*>(row + e0) + i;
+          reinterpret_cast<uint4*>(raw)[i] = kConst ? __ldg(from) : *from;
+        }
       }
 #pragma unroll
       for (int i = 0; i < kPer; ++i) v[i] = score_f32(raw[i]);
@@ -708,7 +710,7 @@ route_backward_kernel(RouteBackwardParams p, bool whole, bool whole_out, bool wh
   }
   float v[kPer], d[kPer], m = 0.f, inv_z = 0.f;
   if (dense) {
-    load_cells<T, kPer>(x, e0, n, whole, v, -INFINITY);
+    load_cells<T, kPer, false>(x, e0, n, whole, v, -INFINITY);  // dlogits may be the logits
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       v[i] = masked(v[i]);

@@ -131,3 +131,26 @@ def test_gradient_of_masked_stays_zero(experts, gpu, torch):  # noqa: F811
                             got = run_backward(torch, gpu, x, ids, dw, ds if dense else None,
                                                score=score, renormalize=renormalize, scale=1.0)
                             assert (got[masked] == 0).all(), (score, renormalize, bad, where)
+
+
+@pytest.mark.parametrize("experts", [24, 64, 100, 128, 256, 500, 1024])
+def test_gradient_in_place_every_form(experts, gpu, torch):  # noqa: F811
+    """Written over the logits, the gradient is the one that is written beside them, whether the
+    call reads whole rows or the chosen experts only."""
+    for dtype in TYPES:
+        for tokens in (1, 77, 3001):
+            x = logits(torch, tokens, experts, dtype, experts + tokens)
+            rng = np.random.default_rng(tokens)
+            ids = torch.topk(x.float(), 4).indices.int()
+            dw = torch.from_numpy(rng.standard_normal((tokens, 4)).astype(np.float32)).cuda()
+            ds = torch.from_numpy(rng.standard_normal((tokens, experts)).astype(np.float32)).cuda()
+            for score in ("softmax", "sigmoid"):
+                for renormalize in (True, False):
+                    for dscores in (None, ds):
+                        how = dict(score=score, renormalize=renormalize, dscores=dscores, stream=0)
+                        want = torch.empty_like(x)
+                        gpu.route_topk_backward(x, ids, dw, want, **how)
+                        got = x.clone()
+                        gpu.route_topk_backward(got, ids, dw, got, **how)
+                        torch.cuda.synchronize()
+                        assert torch.equal(got, want), (dtype, tokens, score, renormalize)
