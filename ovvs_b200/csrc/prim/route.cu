@@ -108,11 +108,14 @@ __device__ __forceinline__ uint32_t image(float v) {
   return static_cast<uint32_t>(u ^ (u >> 31 | static_cast<int>(0x80000000u)));
 }
 
-__device__ __forceinline__ float exp_fast(float x) {  // 2^-22 and the argument's rounding
+// For the choice alone, whose error is counted above: 2^-22 and the argument's rounding, which
+// grows with it.
+__device__ __forceinline__ float exp2_fast(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.44269504f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float exp_fast(float x) { return exp2_fast(x * 1.44269504f); }
 __device__ __forceinline__ float rcp_fast(float x) {  // one unit
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -120,12 +123,27 @@ __device__ __forceinline__ float rcp_fast(float x) {  // one unit
 }
 __device__ __forceinline__ float sigmoid_fast(float x) { return rcp_fast(1.f + exp_fast(-x)); }
 
+// e^x for x <= 0, for what is written: e^x = 2^t e^(x - t ln 2) with t near x / ln 2, and the second
+// factor, which makes up for t's rounding, is 1 + its exponent. Off by the first factor's 4 units
+// of 2^-24, one rounding, and 0.05 |x| for ln 2 as a float: 9 at most. Three instructions more than
+// the above: 1 % of the first case below, 4 of a gradient with all scores; expf cost 8 to 14 in
+// every place. 0 from -104 down and for a NaN.
+__device__ __forceinline__ float exp_down(float x) {
+  x = fmaxf(x, -104.f);
+  const float t = x * 1.44269504f, y = exp2_fast(t);
+  return fmaf(y, fmaf(t, -0.693147182f, x), y);
+}
+__device__ __forceinline__ float sigmoid(float x) {  // 18 units of 2^-24 of itself
+  const float e = exp_down(-fabsf(x)), q = rcp_fast(1.f + e);
+  return x < 0.f ? e * q : q;
+}
+
 // A chosen expert's score over a power of e common to the token's chosen ones, whose largest
 // logit is `top`: their ratios hold where the scores themselves would vanish.
 __device__ __forceinline__ float relative_score(float v, float top, bool sigmoid) {
-  if (!sigmoid) return v == top ? 1.f : exp_fast(v - top);
+  if (!sigmoid) return v == top ? 1.f : exp_down(v - top);
   const float base = fminf(top, 0.f);
-  return rcp_fast(exp_fast(base) + (v == base ? 1.f : exp_fast(base - v)));
+  return rcp_fast(exp_down(base) + (v == base ? 1.f : expf(base - v)));
 }
 
 // The plain way: one warp takes the token, choice and score of each expert in shared memory
@@ -312,37 +330,40 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
   load_cells<T, kPer>(x, e0, n, whole, v, -INFINITY);
   const bool sums = p.groups > 1 && p.group_top2;
   const bool need_scores = kBias || p.scores;
-  float m = 0.f, inv_z = 0.f;
+  const bool scores_out = p.scores || !p.renormalize;  // they are not for the choice alone
+  float s[kPer], m = 0.f, inv_z = 0.f;
   if (!p.sigmoid && (need_scores || sums || !p.renormalize)) {
     m = v[0];  // a NaN is not the larger one
 #pragma unroll
     for (int i = 1; i < kPer; ++i) m = fmaxf(m, v[i]);
     m = lanes_max<kLanes>(fmaxf(m, -INFINITY));
+    if (scores_out) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) s[i] = v[i] == m ? 1.f : exp_down(v[i] - m);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) s[i] = v[i] == m ? 1.f : exp_fast(v[i] - m);
+    }
     float z = 0.f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const float e = v[i] == m ? 1.f : exp_fast(v[i] - m);
-      z += v[i] > -INFINITY ? e : 0.f;
+      s[i] = v[i] > -INFINITY ? s[i] : 0.f;
+      z += s[i];
     }
     z = lanes_sum<kLanes>(z);
     inv_z = z > 0.f ? rcp_fast(z) : 0.f;
   }
-  auto score = [&](float y) {
-    const float s = p.sigmoid ? sigmoid_fast(y) : (y == m ? 1.f : exp_fast(y - m)) * inv_z;
-    return y > -INFINITY ? s : 0.f;
-  };
   uint32_t key[kPer];
   if (need_scores) {
-    float s[kPer];
-    if (p.sigmoid) {
+    if (!p.sigmoid) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) s[i] = v[i] > -INFINITY ? sigmoid_fast(v[i]) : 0.f;
+      for (int i = 0; i < kPer; ++i) s[i] *= inv_z;
+    } else if (scores_out) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) s[i] = v[i] > -INFINITY ? sigmoid(v[i]) : 0.f;
     } else {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const float e = v[i] == m ? 1.f : exp_fast(v[i] - m);
-        s[i] = v[i] > -INFINITY ? e * inv_z : 0.f;
-      }
+      for (int i = 0; i < kPer; ++i) s[i] = v[i] > -INFINITY ? sigmoid_fast(v[i]) : 0.f;
     }
     if (p.scores && live) store_cells<float, kPer>(p.scores + t * n, e0, n, whole_scores, s);
     if constexpr (kBias) {
@@ -398,6 +419,10 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
       if constexpr (kBias) {
         second = second > -INFINITY ? second : 0.f;
       } else {
+        auto score = [&](float y) {
+          const float c = p.sigmoid ? sigmoid_fast(y) : (y == m ? 1.f : exp_fast(y - m)) * inv_z;
+          return y > -INFINITY ? c : 0.f;
+        };
         first = score(first);
         second = score(second);
       }
@@ -644,7 +669,8 @@ route_kernel(RouteParams p, int group_lanes, bool whole, bool whole_scores) {
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
       if (j * kLanes >= k) break;
-      w[j] = score(y[j]);
+      w[j] = p.sigmoid ? sigmoid(y[j]) : (y[j] == m ? 1.f : exp_down(y[j] - m)) * inv_z;
+      w[j] = id[j] >= 0 ? w[j] : 0.f;
     }
   }
   if (live && !plain) {
@@ -729,7 +755,7 @@ route_backward_kernel(RouteBackwardParams p, bool whole, bool whole_out, bool wh
       float z = 0.f;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        v[i] = v[i] > -INFINITY ? (v[i] == m ? 1.f : exp_fast(v[i] - m)) : 0.f;
+        v[i] = v[i] > -INFINITY ? (v[i] == m ? 1.f : exp_down(v[i] - m)) : 0.f;
         z += v[i];
       }
       z = lanes_sum<kLanes>(z);
@@ -765,8 +791,8 @@ route_backward_kernel(RouteBackwardParams p, bool whole, bool whole_out, bool wh
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
       if (j * kLanes >= k) break;
-      const float s = p.sigmoid ? sigmoid_fast(y[j])
-                                : (y[j] == m ? 1.f : exp_fast(y[j] - m)) * inv_z;
+      const float s = p.sigmoid ? sigmoid(y[j])
+                                : (y[j] == m ? 1.f : exp_down(y[j] - m)) * inv_z;
       own[j] = id[j] >= 0 ? s * dw[j] : 0.f;
       if (!p.sigmoid) dot += own[j];
     }
@@ -775,7 +801,7 @@ route_backward_kernel(RouteBackwardParams p, bool whole, bool whole_out, bool wh
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
       if (j * kLanes >= k) break;
-      if (id[j] >= 0) own[j] *= sigmoid_fast(-y[j]);  // 1 - s
+      if (id[j] >= 0) own[j] *= sigmoid(-y[j]);  // 1 - s
     }
   } else if (dense) {
 #pragma unroll
@@ -819,7 +845,7 @@ route_backward_kernel(RouteBackwardParams p, bool whole, bool whole_out, bool wh
   if (dense && p.sigmoid) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const float ex = exp_fast(-fabsf(v[i])), q = rcp_fast(1.f + ex);
+      const float ex = exp_down(-fabsf(v[i])), q = rcp_fast(1.f + ex);
       g[i] += v[i] > -INFINITY ? d[i] * ex * q * q : 0.f;
     }
   } else if (dense) {  // 0 where the score is 0, whatever dot is

@@ -6,9 +6,11 @@ import numpy as np
 import pytest
 
 from tests import rows_reference as ref
-from tests.test_gpu_rows import TYPES, check_route, logits, run_backward, torch  # noqa: F401
+from tests.test_gpu_rows import TINY, TYPES, check_route, logits, run_backward, torch  # noqa: F401
 
 pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24  # half a step of fp32
 
 
 # ---- routing: biases of any size ------------------------------------------------------------------
@@ -154,3 +156,90 @@ def test_gradient_in_place_every_form(experts, gpu, torch):  # noqa: F811
                         gpu.route_topk_backward(got, ids, dw, got, **how)
                         torch.cuda.synchronize()
                         assert torch.equal(got, want), (dtype, tokens, score, renormalize)
+
+
+# ---- accuracy of scores, weights and gradients -----------------------------------------------------
+
+def far_logits(torch, tokens, experts, seed):  # noqa: F811
+    """fp32 logits on a grid of 1/64 within +-60: every difference of two is exact in fp32."""
+    v = np.random.default_rng(seed).integers(-60 * 64, 60 * 64, (tokens, experts)) / 64.0
+    return torch.from_numpy(v.astype(np.float32)).cuda()
+
+
+@pytest.mark.parametrize("experts", [16, 64, 128, 256, 512, 1024])
+def test_scores_far_from_the_largest(experts, gpu, torch):  # noqa: F811
+    """A score's relative error does not grow with its logit. In units of 2^-24: an exponential of
+    an exact argument 9 (the power of two 4, one rounding, and 0.05 a unit of the argument, up to 87
+    of them), its sum over E experts E / 32 additions in a lane, 8 at least, and 5 between lanes, a
+    reciprocal 2, each product, quotient or addition 1. A softmax score: 9 + (9 + E / 32 + 5) + 2 + 1;
+    a sigmoid e / (1 + e): 9, half of them and 1 more below, 2, 1. A weight over the sum of the
+    chosen: a relative score (an exponential of 9 and one of 4, their sum, a reciprocal: 12 at most),
+    12 + 9 of the sum, a reciprocal 2, two products. (Exponentials of rounded arguments, x log2 e in
+    fp32, are off by some 60 at the far end.)"""
+    x = far_logits(torch, 200, experts, experts)
+    xs = x.double().cpu().numpy()
+    for score in ("softmax", "sigmoid"):
+        for renormalize in (True, False):
+            ids = torch.empty(200, 6, dtype=torch.int32, device="cuda")
+            w = torch.empty(200, 6, device="cuda")
+            s = torch.empty(200, experts, device="cuda")
+            gpu.route_topk(x, ids, w, score=score, renormalize=renormalize, scores=s, stream=0)
+            want = ref.route(xs, 6, score=score, renormalize=renormalize)
+            assert np.array_equal(ids.cpu().numpy(), want[0])
+            per = 8 if experts <= 256 else experts / 32
+            tol = (9 + 9 + per + 5 + 2 + 1 if score == "softmax" else 9 + 4.5 + 1 + 2 + 1) * U
+            got = s.double().cpu().numpy()
+            assert np.all(np.abs(got - want[2]) <= tol * want[2] + TINY), (score, "scores")
+            if renormalize:
+                tol = (12 + 12 + 9 + 2 + 2) * U
+            got = w.double().cpu().numpy()
+            assert np.all(np.abs(got - want[1]) <= (tol + U) * want[1] + TINY), (score, "weights")
+
+
+def far_gradient(x, ids, dw, ds, score, renormalize):
+    """(gradient, magnitudes added up for it) of rows without masks, 1 - s taken as 1 / (1 + e^x):
+    from a logit of 37 on, 1 - s itself has no digit left in 64 bits."""
+    s = np.stack([ref.scores_row(row, score) for row in x])
+    rest = 1.0 / (1.0 + np.exp(x)) if score == "sigmoid" else np.ones_like(x)
+    part = np.stack([ref.ratio_row(row, i, score) for row, i in zip(x, ids)])
+    if not renormalize:
+        part = np.take_along_axis(s, ids.astype(np.int64), 1)
+    own, mag = part * dw, part * np.abs(dw)
+    if renormalize:
+        own, mag = part * (dw - own.sum(1, keepdims=True)), mag + part * mag.sum(1, keepdims=True)
+    grad, size = s * ds * rest, s * np.abs(ds) * rest
+    at = np.arange(len(x))[:, None]
+    if score == "softmax":
+        total, most = (s * ds).sum(1, keepdims=True), (s * np.abs(ds)).sum(1, keepdims=True)
+        if not renormalize:
+            total, most = total + own.sum(1, keepdims=True), most + mag.sum(1, keepdims=True)
+        grad, size = grad - s * total, size + s * most
+    grad[at, ids] += own * rest[at, ids]
+    size[at, ids] += mag * rest[at, ids]
+    return grad, size
+
+
+@pytest.mark.parametrize("experts", [16, 64, 256, 1024])
+def test_gradient_far_from_the_largest(experts, gpu, torch):  # noqa: F811
+    """The same of the gradient's terms: a score (softmax 26 + E / 32, sigmoid 18) or a ratio of
+    the chosen (37), 1 - s (18), a sum of products over the experts (E / 32 + 5 additions, a
+    product and a score each), three more products and sums, in units of 2^-24 of the magnitudes
+    added up."""
+    x = far_logits(torch, 60, experts, experts + 1)
+    xs = x.double().cpu().numpy()
+    rng = np.random.default_rng(experts)
+    dw = rng.standard_normal((60, 5)).astype(np.float32)
+    ds = rng.standard_normal((60, experts)).astype(np.float32)
+    per = 8 if experts <= 256 else experts / 32
+    for score in ("softmax", "sigmoid"):
+        ids = ref.route(xs, 5, score=score)[0]
+        for renormalize in (True, False):
+            for dense in (True, False):
+                d = ds if dense else None
+                how = dict(score=score, renormalize=renormalize, scale=1.0)
+                got = run_backward(torch, gpu, x, ids, dw, d, **how)
+                want, size = far_gradient(xs, ids, dw.astype(np.float64), ds.astype(np.float64)
+                                          * dense, score, renormalize)
+                one = max(26 + per, 37)
+                tol = (one + 18 + (per + 5 + 1 + one) + 6) * U
+                assert np.all(np.abs(got - want) <= tol * size + TINY), (score, renormalize, dense)
