@@ -159,8 +159,9 @@ typedef enum ovvsScoreType {
    order with probability 1. A row with every score masked gives id -1, probability 0, kept 0.
    Weights and their sums are 64-bit integers, so that no sum rounds: a weight is a multiple of
    2^-50 of the row's largest up to 4,096 columns, of 2^-45 at 131,072 (one bit fewer for every
-   doubling), and one that rounds to 0 is kept like the others but never drawn, not for u = 0
-   either.
+   doubling), less than one such step from its exponential, and one that rounds to 0 is kept like
+   the others but never drawn, not for u = 0 either. (u times the total, and top_p times the
+   weight, are rounded to 53 bits.)
    d_temperature, d_top_k, d_top_p, d_min_p: [rows], each may be NULL (1, off, off, off).
    d_uniforms [rows x draws]. d_ids [rows x draws]; d_probs [rows x draws] (may be NULL) gets the
    weight of each drawn column over the total that was drawn from; d_kept [rows] (may be NULL)

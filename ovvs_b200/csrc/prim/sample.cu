@@ -13,8 +13,8 @@
 // the row's largest (2^-45 at 131,072 columns) count as zero.
 //
 // What bounds it: for top-k rows HBM and the latency of a dozen dependent steps, otherwise the
-// weights. A weight good to 2^-38 costs ten 64-bit operations, and the GPU does 64 of those a
-// clock and SM: 25.6 million take 14 us, where reading them as fp16 takes 8.
+// weights. A weight good to 2^-51 costs twelve 64-bit operations, and the GPU does 64 of those a
+// clock and SM: 25.6 million take 17 us, where reading them as fp16 takes 8.
 //
 // One cluster of blocks takes one row. Each block holds its columns in shared memory, so the row
 // is read from HBM once and every later look at it costs shared memory only; what a block cannot
@@ -84,9 +84,11 @@ __constant__ double kSixteenths[16] = {
     1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
 
 // Weights of one row. 2^(t / 16) = 2^(n >> 4) * 2^((n & 15) / 16) * 2^(f / 16) with n = round(t),
-// the last factor by the polynomial of degree 4 through its values at the Chebyshev points of
-// [-1/2, 1/2], which is 2^-38.5 off at most: ten 64-bit operations a weight, where the power
-// function takes some forty. The result is rounded to an integer by adding 2^52.
+// the last factor by the polynomial of degree 6 through its values at the Chebyshev points of
+// [-1/2, 1/2], which is 2^-56.8 off at most: twelve 64-bit operations a weight, where the power
+// function takes some forty. With the table's rounding and the polynomial's own, p * scaled is off
+// by 3 * 2^-53 of itself, under half a step of the finest grid, 2^-50. The result is rounded to an
+// integer by adding 2^52.
 struct Weigher {
   double m, rate;  // max; 16 log2(e) / T
   float cut;       // scores below it weigh 0
@@ -110,10 +112,10 @@ struct Weigher {
     const double r = fma(d, rate, magic);
     const int n = __double2loint(r);
     const double f = fma(d, rate, magic - r);
-    double p = fma(f, 1.4676387238435006e-07, 1.3551205154935067e-05);
-    p = fma(f, p, 0.0009383847926296646);
-    p = fma(f, p, 0.043321698760160544);
-    p = fma(f, p, 1.0);
+    const double f2 = f * f;
+    double p = fma(f2, 9.181354192172116e-12, fma(f, 1.2716120543851127e-09, 1.4676100321236697e-07));
+    p = fma(f2, p, fma(f, 1.3550807776390032e-05, 0.0009383847928089877));
+    p = fma(f2, p, fma(f, 0.04332169878499668, 1.0));
     const double s = table[n & 15];
     const double scaled = __hiloint2double(__double2hiint(s) + (n & ~15) * (1 << 16),
                                            __double2loint(s));

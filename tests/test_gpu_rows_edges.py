@@ -6,7 +6,8 @@ import numpy as np
 import pytest
 
 from tests import rows_reference as ref
-from tests.test_gpu_rows import TINY, TYPES, check_route, logits, run_backward, torch  # noqa: F401
+from tests.test_gpu_rows import (  # noqa: F401
+    TINY, TYPES, check_route, logits, run_backward, run_sample, torch)
 
 pytestmark = pytest.mark.gpu
 
@@ -243,3 +244,42 @@ def test_gradient_far_from_the_largest(experts, gpu, torch):  # noqa: F811
                 one = max(26 + per, 37)
                 tol = (one + 18 + (per + 5 + 1 + one) + 6) * U
                 assert np.all(np.abs(got - want) <= tol * size + TINY), (score, renormalize, dense)
+
+
+# ---- accuracy of a draw's weights ------------------------------------------------------------------
+
+def borders(lowest, highest, count=1 << 23):
+    """Scores x (fp32, beside a score of 0) and uniforms u = j / 2^24 whose distance from
+    w / (w + 1), w = exp(x), lies between the two powers of two; and which side u is on. In 80-bit
+    arithmetic, whose 2^-63 is far below the distances."""
+    x = (-3 * np.random.default_rng(9).random(count, dtype=np.float32)).astype(np.float32)
+    w = np.exp(x.astype(np.longdouble))
+    f = w / (w + 1)
+    j = np.rint(f * 2 ** 24)
+    off = np.abs(f - j / np.longdouble(2 ** 24))
+    at = np.flatnonzero((off > 2.0 ** lowest) & (off < 2.0 ** highest))
+    return x[at], (j[at] / 2 ** 24).astype(np.float32), (f[at] <= j[at] / 2 ** 24).astype(np.int64)
+
+
+def test_draws_next_to_a_border(gpu, torch):  # noqa: F811
+    """Weights are exact to their grid: 2^-50 of the largest up to 4,096 columns, and a draw's
+    border is off by no more. Two columns' w / (w + 1) is off by what w is off, so a border 2^-48
+    away has to be seen from its right side. (A weight good to 2^-38 sees most of them from
+    either.)"""
+    assert np.finfo(np.longdouble).nmant >= 63
+    x, u, want = borders(-48, -41)
+    assert len(x) > 30 and 5 < want.sum() < len(x) - 5
+    rows = torch.zeros(len(x), 2, device="cuda")
+    rows[:, 0] = torch.from_numpy(x)
+    ids = run_sample(torch, gpu, rows, u[:, None])[0][:, 0]
+    assert np.array_equal(ids, want)
+    # the same two columns far apart in a long row of nothing else: a cluster of blocks, and a grid
+    # of 2^-47 of the largest
+    x, u, want = borders(-45, -39)
+    assert len(x) > 100
+    rows = torch.full((len(x), 30000), -float("inf"), device="cuda")
+    rows[:, 77] = torch.from_numpy(x)
+    rows[:, 29000] = 0.0
+    for part in range(0, len(x), 40):  # not a batch that one block a row takes
+        ids = run_sample(torch, gpu, rows[part:part + 40], u[part:part + 40, None])[0][:, 0]
+        assert np.array_equal(ids, np.where(want[part:part + 40] == 0, 77, 29000))
