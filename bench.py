@@ -342,6 +342,61 @@ def _parity(nb, ds, nb_ref, ds_ref, rtol):
     return out
 
 
+def _reference_missing():
+    """Why the reference library cannot be run here (one line), or None where it can."""
+    from oracle import cpu
+
+    if os.path.exists(cpu.REFERENCE_SO):
+        return None
+    return ("oracle/_ref/libovvs_ref.so is not built: it is compiled from the reference's own "
+            "sources, and no reference checkout was there")
+
+
+RESTATEMENT = ("this repository's CPU restatement of the reference (oracle/ovvs_oracle.cpp; the "
+               "reference library itself is not built here), ")
+
+
+def _oracle_sample(cfg, data_host, q_host, n_queries):
+    """(neighbours, distances) of the first n_queries queries by the CPU restatement, shard by
+    shard of 1M rows like _reference_sample; not timed."""
+    from oracle.cpu import Oracle
+
+    o = Oracle()
+    qs = np.ascontiguousarray(q_host[:n_queries], np.float32)
+    parts = []
+    for s0 in range(0, cfg["n"], CHUNK):
+        shard = np.ascontiguousarray(data_host[s0: s0 + CHUNK])
+        ks = min(cfg["k"], shard.shape[0])
+        nb, ds = o.brute_search(o.convert_to_f32(cfg["dtype"], shard), qs, cfg["k"], cfg["metric"])
+        parts.append((nb[: n_queries * ks].reshape(n_queries, ks) + s0,
+                      ds[: n_queries * ks].reshape(n_queries, ks)))
+    return _merge_shard_topk(parts, min(cfg["k"], cfg["n"]), cfg["metric"] == "inner_product")
+
+
+def _search_baseline(cfg, data_host, q_host, nb, ds, seconds):
+    """The CPU baseline and the parity block of a search config, for this library's results nb,
+    ds [nq, k] on q_host: against the reference library, timed, or, where that is not built,
+    against the CPU restatement and without a baseline."""
+    threads, nq_s = _reference_sizes(cfg, seconds)
+    missing = _reference_missing()
+    if missing is None:
+        secs, nb_ref, ds_ref = _reference_sample(cfg, data_host, q_host, threads, nq_s)
+        baseline = {
+            "value": nq_s / secs, "unit": "queries/s", "cores": threads, "kind": "reference",
+            "sample": f"{nq_s} queries x all {cfg['n']} rows: the reference library built from "
+                      f"its sources (oracle/_ref), FORCE_CPU, 1M-row shards, {threads} threads"}
+        against = "the reference library (oracle/_ref), FORCE_CPU, same queries"
+    else:
+        nb_ref, ds_ref = _oracle_sample(cfg, data_host, q_host, nq_s)
+        baseline = {"value": None, "unavailable": missing}
+        against = RESTATEMENT + "same queries"
+    # The same sampled queries' results from the timed runs, against the checker's.
+    parity = _parity(nb[:nq_s], ds[:nq_s], nb_ref, ds_ref,
+                     2e-3 if cfg["dtype"] == "f16" else 1e-4)
+    parity["against"] = against
+    return {"cpu_baseline": baseline, "parity": parity}
+
+
 def _reference_sample(cfg, data_host, q_host, threads, n_queries):
     """Times the reference's FORCE_CPU ovvsBruteForceSearch on `n_queries` queries against all
     rows: row shards of 1M, `threads` host threads per shard (one Resources each, sharing the
@@ -673,23 +728,12 @@ def run_ours(args, cfg):
         dist.destroy_process_group()
 
     if rank == 0 and world == 1 and not args.no_cpu_baseline:
-        threads, nq_s = _reference_sizes(cfg, args.ref_seconds)
-        data_host = shard_host
-        secs, nb_ref, ds_ref = _reference_sample(cfg, data_host, q_host, threads, nq_s)
-        line["cpu_baseline"] = {
-            "value": nq_s / secs, "unit": "queries/s", "cores": threads, "kind": "reference",
-            "sample": f"{nq_s} queries x all {n} rows: the reference library built from its "
-                      f"sources (oracle/_ref), FORCE_CPU, 1M-row shards, {threads} threads"}
-        # The same sampled queries' results from the timed runs above, against the reference's.
-        parity = _parity(nb_h[: nq_s * k_eff].reshape(nq_s, k_eff),
-                         ds_h[: nq_s * k_eff].reshape(nq_s, k_eff), nb_ref, ds_ref,
-                         2e-3 if cfg["dtype"] == "f16" else 1e-4)
-        parity["against"] = "the reference library (oracle/_ref), FORCE_CPU, same queries"
-        line["parity"] = parity
+        line.update(_search_baseline(cfg, shard_host, q_host, nb_h[: nq * k_eff].reshape(nq, k_eff),
+                                     ds_h[: nq * k_eff].reshape(nq, k_eff), args.ref_seconds))
     if rank == 0:
         print(json.dumps(line), flush=True)
         if "parity" in line and not line["parity"]["ok"]:
-            print("parity FAILED against the reference", file=sys.stderr)
+            print("parity FAILED: " + line["parity"]["against"], file=sys.stderr)
             return 1
     return 0
 
@@ -814,11 +858,22 @@ def run_kmeans(args, cfg):
         dist.destroy_process_group()
     if rank == 0 and world == 1 and not args.no_cpu_baseline:
         rows = _reference_kmeans_rows(cfg, args.ref_seconds)
-        ref_out = {}
-        secs, it = _reference_kmeans_sample(cfg, shard_host, rows, ref_out)
-        value, sample = _reference_kmeans_line(args, cfg, [secs], rows, it)
-        line["cpu_baseline"] = {"value": value, "unit": "iterations/s", "cores": 1,
-                                "kind": "reference", "sample": sample}
+        missing = _reference_missing()
+        if missing is None:
+            ref_out = {}
+            secs, it = _reference_kmeans_sample(cfg, shard_host, rows, ref_out)
+            value, sample = _reference_kmeans_line(args, cfg, [secs], rows, it)
+            line["cpu_baseline"] = {"value": value, "unit": "iterations/s", "cores": 1,
+                                    "kind": "reference", "sample": sample}
+            ref_c = ref_out["centroids"]
+            against = "the reference library (oracle/_ref), FORCE_CPU, same rows"
+        else:
+            from oracle.cpu import Oracle
+
+            it = 4
+            ref_c = Oracle().kmeans_fit(np.ascontiguousarray(shard_host[:rows], np.float32), C, it)
+            line["cpu_baseline"] = {"value": None, "unavailable": missing}
+            against = RESTATEMENT + "same rows"
         # The same fit on this library (same rows, clusters and iterations; both seed with the
         # reference's mt19937(42) row sample): centroids must be bit-identical.
         res = ov.Resources.sharded(local, 0, 1, None)
@@ -827,7 +882,6 @@ def run_kmeans(args, cfg):
         ours = m.centroids()
         m.close()
         res.close()
-        ref_c = ref_out["centroids"]
         same = (ours.shape == ref_c.shape and
                 np.array_equal(ours.view(np.uint32), ref_c.view(np.uint32)))
         rel = float(np.max(np.abs(ours.astype(np.float64) - ref_c) /
@@ -835,12 +889,11 @@ def run_kmeans(args, cfg):
             if ours.shape == ref_c.shape else float("inf")
         line["parity"] = {"rows": rows, "clusters": C, "iters": it,
                           "centroids_bit_identical": bool(same), "max_rel_err": rel,
-                          "ok": bool(same),
-                          "against": "the reference library (oracle/_ref), FORCE_CPU, same rows"}
+                          "ok": bool(same), "against": against}
     if rank == 0:
         print(json.dumps(line), flush=True)
         if "parity" in line and not line["parity"]["ok"]:
-            print("parity FAILED against the reference", file=sys.stderr)
+            print("parity FAILED: " + line["parity"]["against"], file=sys.stderr)
             return 1
     return 0
 
@@ -1055,7 +1108,9 @@ def run_ivf(args, cfg):
             "clocks": {"sm_mhz": clk["sm_mhz"], "sm_max_mhz": clk["sm_max_mhz"],
                        "reasons": clk["reasons"]},
         }
-        if world == 1 and not args.no_cpu_baseline:
+        if world == 1 and not args.no_cpu_baseline and _reference_missing():
+            line["cpu_baseline"] = {"value": None, "unavailable": _reference_missing()}
+        elif world == 1 and not args.no_cpu_baseline:
             threads, nq_s = _ivf_reference_sizes(cfg, args.ref_seconds)
             secs = _ivf_reference_search(path, q_host, cfg, threads, nq_s)
             line["cpu_baseline"] = {
@@ -1233,24 +1288,31 @@ def run_prim(args, cfg):
                        "reasons": clk["reasons"]},
         }
         if world == 1 and not args.no_cpu_baseline:
-            from oracle.cpu import Reference
+            from oracle.cpu import Oracle, Reference
 
-            ref = Reference()
+            missing = _reference_missing()
+            ref = Reference() if missing is None else Oracle()
             rows = _prim_reference_rows(cfg, args.ref_seconds)
             xs = np.ascontiguousarray(x[:rows])
             t0 = time.perf_counter()
             ref_out = np.asarray(_prim_call(ref, cfg, xs, y), np.float32).reshape(rows, ny)
             secs = time.perf_counter() - t0
-            line["cpu_baseline"] = {
-                "value": rows * ny / secs, "unit": "outputs/s", "cores": 1, "kind": "reference",
-                "sample": f"{rows} of {nx} rows x all {ny} through the reference library built "
-                          "from its sources (oracle/_ref), FORCE_CPU (its naive loop is "
-                          "single-threaded)"}
+            if missing is None:
+                line["cpu_baseline"] = {
+                    "value": rows * ny / secs, "unit": "outputs/s", "cores": 1,
+                    "kind": "reference",
+                    "sample": f"{rows} of {nx} rows x all {ny} through the reference library "
+                              "built from its sources (oracle/_ref), FORCE_CPU (its naive loop "
+                              "is single-threaded)"}
+                against = "the reference library (oracle/_ref), FORCE_CPU"
+            else:
+                line["cpu_baseline"] = {"value": None, "unavailable": missing}
+                against = RESTATEMENT + "same operands"
             got = np.asarray(out, np.float32).reshape(nx, ny)[:rows]
             same = got.view(np.uint32) == ref_out.view(np.uint32)
             line["parity"] = {"rows": rows, "outputs": int(same.size),
                               "bit_identical": int(same.sum()), "ok": bool(same.all()),
-                              "against": "the reference library (oracle/_ref), FORCE_CPU"}
+                              "against": against}
     res.close()
     if world > 1:
         dist.barrier()
@@ -1314,6 +1376,11 @@ def main():
         args.warmup = 3
     cfg = CONFIGS[args.config]
     if args.impl == "reference":
+        missing = _reference_missing()
+        if missing is not None:
+            if int(os.environ.get("RANK", "0")) == 0:
+                print(json.dumps({"impl": "reference", "unavailable": missing}), flush=True)
+            return 0
         if cfg.get("kind") == "ivf":
             return run_ivf_reference(args, cfg)
         if cfg.get("kind") == "prim":
