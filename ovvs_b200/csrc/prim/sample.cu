@@ -24,8 +24,8 @@
 //     pass. Those go to block 0, which orders and draws; the other blocks are done. In large
 //     batches one block takes the row, holds nothing, finds the bound in a part of it and lists
 //     what reaches it as it streams by. 1000 rows of 100,000 fp32, top-100, 64 draws: 108 us, the
-//     400 MB at 3.7 TB/s (a block either loads or orders, and 740 of the 1000
-//     rows are under way at once); one row of 32,000: 8.8 us.
+//     400 MB at 3.7 TB/s (a block either loads or orders, five an SM: 740 of the 1000 rows are
+//     under way at once); one row of 32,000: 8.8 us.
 //   - anything else: the edge of top-p is bracketed by a histogram of the weights over
 //     (m - x) / T, the few columns in the bracket are ordered by block 0, the weights above it
 //     are summed exactly. The draw walks the columns of the warp whose range of running sums
@@ -563,11 +563,21 @@ __device__ void finish_list(const SampleParams& p, int64_t row, int n, const Set
   }
 }
 
-// kBlocks: blocks an SM is meant to hold. Where one block takes a row, five of 48 registers a
-// thread stream better than four of 64 (1000 rows of 100,000 fp32, top-100: 113 us against 134).
-// Where a cluster does, the weights want the registers: four of 64 in a large batch (256 rows of
-// 100,003 fp16, top-p: 168 us, three of 80: 182, five of 48: 197), three in one that leaves the
-// SMs room (64 rows of 131,072 fp32, mixed: 54 us against 62).
+// kBlocks: blocks an SM can hold by their registers. Where one block takes a row, five of 48
+// registers a thread, and kOneBlock of shared memory each. Their loads on the way stand in what
+// shared memory leaves of the SM's 256 KB, so that this must be little: 1000 rows of 100,000 fp32,
+// top-100, take 108 us with five blocks of 38 KB (60 KB left), 107 with 30 KB, 109 with four of 45,
+// but 134 with five of 44 KB or four of 56 (28 left). The fifth block is worth 2 to 5 % to rows
+// that are gone through several times.
+// Where a cluster takes a row, the weights want the registers: four of 64 in a large batch (256
+// rows of 100,003 fp16, top-p: 168 us, three of 80: 182, five of 48: 197), three of 80 in one that
+// leaves the SMs room (64 rows of 131,072 fp32, mixed: 54 us against 62). How many stand on an SM
+// is then often said by the part of the row that they hold: of that last case's blocks, 89 KB each,
+// two, so that 37 of its 64 clusters run at once. Three or four that hold less of it and read the
+// rest again take longer (67 us against 57).
+constexpr int kOneBlock = 38 * 1024;
+static_assert(5 * (kOneBlock + 1024) <= 196 * 1024, "five blocks, and 60 KB beside them");
+static_assert(kOneBlock >= sizeof(Shared) + 4096, "and room to hold some chunks");
 template <class T, int kBlocks>
 __global__ void __launch_bounds__(kThreads, kBlocks)
 sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
@@ -1260,7 +1270,7 @@ cudaError_t sample(const SampleParams& p, cudaStream_t stream) {
   // A batch of two rows an SM or more that may have top-k rows goes one block a row, which reads a
   // top-k row in one pass (512 rows of 100,003 fp16, top-50: 32 us against 86 by clusters of 8;
   // rows under top-p alone, which it reads again from L2, take 354 against 296). Otherwise a row
-  // gets a cluster: as many blocks as the SMs hold three of, of 512 chunks or more (16 rows of
+  // gets a cluster: up to three blocks an SM over all rows, of 512 chunks or more (16 rows of
   // 32,000 bf16, top-p: 25 us by 8 blocks, 40 by 2), and beyond that as few as keep a block's
   // part at 2048 chunks (400 such rows: 138 us by 8 blocks, 90 by 2, 112 by 1).
   const bool one_pass = p.top_k && p.rows >= 296;
@@ -1269,7 +1279,7 @@ cudaError_t sample(const SampleParams& p, cudaStream_t stream) {
          (p.rows * nb * 2 <= 444 || chunks / nb > 2048))
     nb *= 2;
   const int block_chunks = static_cast<int>((chunks + nb - 1) / nb);
-  const int most = static_cast<int>(((one_pass ? 45 : 227) * 1024 - kFixed) / 16);
+  const int most = static_cast<int>(((one_pass ? kOneBlock : 227 * 1024) - kFixed) / 16);
   const int resident = block_chunks < most ? block_chunks : most;
   const int way = one_pass ? 2 : p.rows * nb > 592;
   auto kernel = way == 2 ? sample_kernel<T, 5> : way ? sample_kernel<T, 4> : sample_kernel<T, 3>;
