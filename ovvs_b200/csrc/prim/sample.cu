@@ -23,8 +23,8 @@
 //     warps' best maxima bounds the k-th score from below and lets little more than k columns
 //     pass. Those go to block 0, which orders and draws; the other blocks are done. In large
 //     batches one block takes the row, holds nothing, finds the bound in a part of it and lists
-//     what reaches it as it streams by. 1000 rows of 100,000 fp32, top-100, 64 draws: 108 us, the
-//     400 MB at 3.7 TB/s (a block either loads or orders, five an SM: 740 of the 1000 rows are
+//     what reaches it as it streams by. 1000 rows of 100,000 fp32, top-100, 64 draws: 103 us, the
+//     400 MB at 3.9 TB/s (a block either loads or orders, four an SM: 592 of the 1000 rows are
 //     under way at once); one row of 32,000: 8.8 us.
 //   - anything else: the edge of top-p is bracketed by a histogram of the weights over
 //     (m - x) / T, the few columns in the bracket are ordered by block 0, the weights above it
@@ -563,12 +563,12 @@ __device__ void finish_list(const SampleParams& p, int64_t row, int n, const Set
   }
 }
 
-// kBlocks: blocks an SM can hold by their registers. Where one block takes a row, five of 48
+// kBlocks: blocks an SM can hold by their registers. Where one block takes a row, four of 64
 // registers a thread, and kOneBlock of shared memory each. Their loads on the way stand in what
 // shared memory leaves of the SM's 256 KB, so that this must be little: 1000 rows of 100,000 fp32,
-// top-100, take 108 us with five blocks of 38 KB (60 KB left), 107 with 30 KB, 109 with four of 45,
-// but 134 with five of 44 KB or four of 56 (28 left). The fifth block is worth 2 to 5 % to rows
-// that are gone through several times.
+// top-100, take 103 us with four blocks of 38 KB (92 KB left), 105 with 46, but 131 with 56 (28
+// left). A fifth block, for 48 registers, spills and brings nothing: 107 us with 38 KB, 134 with
+// 44; rows of that batch under top-p alone 905 us against 835.
 // Where a cluster takes a row, the weights want the registers: four of 64 in a large batch (256
 // rows of 100,003 fp16, top-p: 168 us, three of 80: 182, five of 48: 197), three of 80 in one that
 // leaves the SMs room (64 rows of 131,072 fp32, mixed: 54 us against 62). How many stand on an SM
@@ -576,7 +576,7 @@ __device__ void finish_list(const SampleParams& p, int64_t row, int n, const Set
 // two, so that 37 of its 64 clusters run at once. Three or four that hold less of it and read the
 // rest again take longer (67 us against 57).
 constexpr int kOneBlock = 38 * 1024;
-static_assert(5 * (kOneBlock + 1024) <= 196 * 1024, "five blocks, and 60 KB beside them");
+static_assert(4 * (kOneBlock + 1024) <= 164 * 1024, "four blocks, and 92 KB beside them");
 static_assert(kOneBlock >= sizeof(Shared) + 4096, "and room to hold some chunks");
 template <class T, int kBlocks>
 __global__ void __launch_bounds__(kThreads, kBlocks)
@@ -1281,10 +1281,10 @@ cudaError_t sample(const SampleParams& p, cudaStream_t stream) {
   const int block_chunks = static_cast<int>((chunks + nb - 1) / nb);
   const int most = static_cast<int>(((one_pass ? kOneBlock : 227 * 1024) - kFixed) / 16);
   const int resident = block_chunks < most ? block_chunks : most;
-  const int way = one_pass ? 2 : p.rows * nb > 592;
-  auto kernel = way == 2 ? sample_kernel<T, 5> : way ? sample_kernel<T, 4> : sample_kernel<T, 3>;
-  static std::atomic<uint64_t> done[3];
-  const cudaError_t e = allow_smem(kernel, 227 * 1024, done[way]);
+  const bool many = one_pass || p.rows * nb > 592;
+  auto kernel = many ? sample_kernel<T, 4> : sample_kernel<T, 3>;
+  static std::atomic<uint64_t> done[2];
+  const cudaError_t e = allow_smem(kernel, 227 * 1024, done[many]);
   if (e != cudaSuccess) return e;
   const LaunchShape shape{static_cast<unsigned>(p.rows * nb), kThreads,
                           kFixed + static_cast<size_t>(resident) * 16, static_cast<unsigned>(nb)};
