@@ -1046,12 +1046,14 @@ sample_kernel(SampleParams p, int frac, int block_chunks, int resident) {
     const u64 in = edge;
     // Bins of (m - x) / T. The edge's weight is at least (1 - p) / cols of the largest, so they
     // reach that far and no further: 100 to 200 a unit. A bin sums weights relative to its upper
-    // end, in 1 / unit, from a second-order series: good to half a unit and 1e-6.
+    // end, in 1 / unit, from a second-order series: good to half a unit and 1e-6. The unit is a
+    // whole number, so that the rounded parts of a block's columns stay below 2^32 together.
     const float reach_units = logf(static_cast<float>(cols) / (1.f - fmaxf(o.tp, 0.f))) + 0.1f;
     const float bins_per_unit = kBins / reach_units;
     const float per_unit = bins_per_unit / t;
     const bool binned = !w.top_inf && per_unit > 0.f && per_unit < INFINITY;
-    const float unit = fminf(65536.f, 4294967040.f / (static_cast<float>(block_chunks) * C::kN));
+    const float unit =
+        floorf(fminf(65536.f, 4294966016.f / (static_cast<float>(block_chunks) * C::kN)));
     unsigned* hist = reinterpret_cast<unsigned*>(sh.wts);
     float* hist_total = reinterpret_cast<float*>(sh.pre);
     for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;

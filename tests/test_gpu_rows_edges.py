@@ -7,7 +7,7 @@ import pytest
 
 from tests import rows_reference as ref
 from tests.test_gpu_rows import (  # noqa: F401
-    TINY, TYPES, check_route, logits, run_backward, run_sample, torch)
+    TINY, TYPES, check_route, check_sample, logits, run_backward, run_sample, torch)
 
 pytestmark = pytest.mark.gpu
 
@@ -283,3 +283,30 @@ def test_draws_next_to_a_border(gpu, torch):  # noqa: F811
     for part in range(0, len(x), 40):  # not a batch that one block a row takes
         ids = run_sample(torch, gpu, rows[part:part + 40], u[part:part + 40, None])[0][:, 0]
         assert np.array_equal(ids, np.where(want[part:part + 40] == 0, 77, 29000))
+
+
+def test_top_p_over_blocks_of_equal_scores(gpu, torch):  # noqa: F811
+    """A long row whose first part is one score, so often that its parts in the histogram that
+    brackets the edge come near 2^32: the edge, among the different scores behind, is right, and
+    is found by its bracket. That shows in the time alone: by the long way a row takes twice as
+    long, so that the least of several times is compared with that of a row 1 % shorter whose parts
+    stay clear of 2^32 however they are rounded."""
+    how = dict(top_p=[0.999, 0.99997])
+    times = {}
+    for cols in (540000, 544001, 584011, 592013):
+        x = logits(torch, 2, cols, "float32", cols, 1.0)
+        x[:, :cols // 8 + 8] = 6.0
+        u = np.array([[0.01, 0.5, 0.93, 0.99999]] * 2, np.float32)
+        check_sample(torch, gpu, x, u, **how)
+        top_p = torch.tensor(how["top_p"], device="cuda")
+        ud, ids = torch.from_numpy(u).cuda(), torch.empty(2, 4, dtype=torch.int64, device="cuda")
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        least = []
+        for _ in range(10):
+            a.record()
+            gpu.sample_rows(x, ud, ids, top_p=top_p, stream=0)
+            b.record()
+            torch.cuda.synchronize()
+            least.append(a.elapsed_time(b))
+        times[cols] = min(least)
+    assert all(t < 1.5 * times[540000] for t in times.values()), times
