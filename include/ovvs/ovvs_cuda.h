@@ -128,7 +128,9 @@ OVVS_API ovvsStatus ovvsIvfFlatSearchDevice(ovvsResources_t res, ovvsIvfFlatInde
 
 /* The drawn and the trained counterparts of ovvsTopk, for scores that are already on the GPU: a
    search's scores, a router's or a language model's logits. All pointers are device pointers on
-   the Resources' device, aligned to their element; sizes have to be positive. Each call checks
+   the Resources' device, aligned to their element; sizes have to be positive (rows or tokens up to
+   134,217,712). An output lies neither where another does nor where an input does, but for the
+   gradient that is written over its logits. Each call checks
    its arguments (INVALID_ARGUMENT, or SHAPE_MISMATCH where a size is beyond a limit), enqueues
    its kernels on `stream` (NULL = the default stream) and returns; it uses no workspace and takes
    no lock, so calls may run at once and may be captured into CUDA graphs. The caller's current

@@ -7,10 +7,14 @@
 
 #include "../prim/rows.cuh"
 #include "ovvs/ovvs_cuda.h"
+#include "overlap.hpp"
 #include "runtime.hpp"
 
 using ovvs::rt::Resources;
+using ovvs::rt::clash;
 using ovvs::rt::from_handle;
+using ovvs::rt::Span;
+using ovvs::rt::span_of;
 
 namespace {
 
@@ -36,11 +40,14 @@ class DeviceScope {
   int before_ = -1;
 };
 
+// `shared`: an output lies where another or an input does. The kernels read and write in no order
+// that a caller could rely on, and the plan's places come from counts of ids that must not change.
 template <class F>
-ovvsStatus launched(Resources& r, F&& launch) {
+ovvsStatus launched(Resources& r, bool shared, F&& launch) {
   try {
     DeviceScope scope;
     OVVS_TRY(scope.enter(r));
+    if (shared) return OVVS_STATUS_INVALID_ARGUMENT;
     const cudaError_t e = launch();
     if (e != cudaSuccess) {
       (void)cudaGetLastError();  // a refused launch is reported once, by this call
@@ -105,7 +112,12 @@ ovvsStatus ovvsSampleRowsDevice(ovvsResources_t res, const void* d_logits, int32
   p.ids = d_ids;
   p.probs = d_probs;
   p.kept = d_kept;
-  return launched(*from_handle(res), [&] {
+  const bool shared = clash(
+      {span_of(d_ids, rows * draws, 8), span_of(d_probs, rows * draws, 4), span_of(d_kept, rows, 4)},
+      {span_of(d_logits, rows, cols, ld, type_bytes(type)), span_of(d_uniforms, rows * draws, 4),
+       span_of(d_temperature, rows, 4), span_of(d_top_k, rows, 4), span_of(d_top_p, rows, 4),
+       span_of(d_min_p, rows, 4)});
+  return launched(*from_handle(res), shared, [&] {
     return ovvs::prim::launch_sample_rows(p, type, static_cast<cudaStream_t>(stream));
   });
 }
@@ -141,7 +153,11 @@ ovvsStatus ovvsRouteTopkDevice(ovvsResources_t res, const void* d_logits, int32_
   p.ids = d_ids;
   p.weights = d_weights;
   p.scores = d_scores;
-  return launched(*from_handle(res), [&] {
+  const bool shared = clash(
+      {span_of(d_ids, tokens * k, 4), span_of(d_weights, tokens * k, 4),
+       span_of(d_scores, tokens * experts, 4)},
+      {span_of(d_logits, tokens, experts, ld, type_bytes(type)), span_of(d_bias, experts, 4)});
+  return launched(*from_handle(res), shared, [&] {
     return ovvs::prim::launch_route_topk(p, type, static_cast<cudaStream_t>(stream));
   });
 }
@@ -173,7 +189,14 @@ ovvsStatus ovvsRouteTopkBackwardDevice(ovvsResources_t res, const void* d_logits
   p.dscores = d_dscores;
   p.dlogits = d_dlogits;
   p.ldd = ldd;
-  return launched(*from_handle(res), [&] {
+  // the logits' own memory, row for row, is allowed
+  const bool in_place = d_dlogits == d_logits && (ldd == ld || tokens == 1);
+  const Span out = span_of(d_dlogits, tokens, experts, ldd, type_bytes(type));
+  const bool shared = clash(
+      {out}, {in_place ? Span{} : span_of(d_logits, tokens, experts, ld, type_bytes(type)),
+              span_of(d_ids, tokens * k, 4), span_of(d_dweights, tokens * k, 4),
+              span_of(d_dscores, tokens * experts, 4)});
+  return launched(*from_handle(res), shared, [&] {
     return ovvs::prim::launch_route_topk_backward(p, type, static_cast<cudaStream_t>(stream));
   });
 }
@@ -191,7 +214,10 @@ ovvsStatus ovvsRoutePlanDevice(ovvsResources_t res, const int32_t* d_ids, int64_
   // every expert that has a pair may leave align - 1 places of its last tile empty
   if (capacity < pairs + (experts < pairs ? experts : pairs) * (int64_t{align} - 1))
     return OVVS_STATUS_SHAPE_MISMATCH;
-  return launched(*from_handle(res), [&] {
+  const bool shared = clash({span_of(d_offsets, experts + 1, 4), span_of(d_order, capacity, 4),
+                             span_of(d_position, pairs, 4)},
+                            {span_of(d_ids, pairs, 4)});
+  return launched(*from_handle(res), shared, [&] {
     return ovvs::prim::launch_route_plan(d_ids, pairs, static_cast<int>(experts), align,
                                          d_offsets, d_order, capacity, d_position,
                                          static_cast<cudaStream_t>(stream));

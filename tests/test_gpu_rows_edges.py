@@ -310,3 +310,49 @@ def test_top_p_over_blocks_of_equal_scores(gpu, torch):  # noqa: F811
             least.append(a.elapsed_time(b))
         times[cols] = min(least)
     assert all(t < 1.5 * times[540000] for t in times.values()), times
+
+
+# ---- outputs over inputs ---------------------------------------------------------------------------
+
+def test_outputs_over_inputs_are_refused(ovvs, gpu, torch):  # noqa: F811
+    x = logits(torch, 6, 64, "float32", 1)
+    u = torch.rand(6, 2, device="cuda")
+    i64 = torch.empty(6, 2, dtype=torch.int64, device="cuda")
+    kept = torch.full((6,), 3, dtype=torch.int32, device="cuda")
+    ids = torch.topk(x, 4).indices.int()
+    w = torch.rand(6, 4, device="cuda")
+    before = [t.clone() for t in (x, u, ids, w)]
+    cut = [t.flatten()[:n].view(s) for t, n, s in ((x, 12, (6, 2)), (x, 24, (6, 4)))]
+    plan = torch.empty(65, dtype=torch.int32, device="cuda")
+    order = torch.empty(24, dtype=torch.int32, device="cuda")
+    calls = [
+        lambda: gpu.sample_rows(x, u, i64, probs=u, stream=0),
+        lambda: gpu.sample_rows(x, u, i64, probs=cut[0], stream=0),
+        lambda: gpu.sample_rows(x, u, i64, kept=kept, top_k=kept, stream=0),
+        lambda: gpu.route_topk(x, ids, w, scores=x, stream=0),
+        lambda: gpu.route_topk(x, ids, ids.view(torch.float32), stream=0),
+        lambda: gpu.route_topk(x, ids, cut[1], stream=0),
+        lambda: gpu.route_topk_backward(x[:5], ids[:5], w[:5], x[1:], stream=0),
+        lambda: gpu.route_topk_backward(x, ids, w, x.flatten()[:192].view(6, 32)
+                                        .as_strided((6, 64), (64, 1), 0), dscores=x, stream=0),
+        lambda: gpu.route_plan(ids, 64, plan, order, ids, stream=0),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(ovvs.OvvsError, match="invalid argument"):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, (x, u, ids, w)))
+
+
+def test_column_ranges_of_one_buffer_are_taken(gpu, torch):  # noqa: F811
+    """Logits and their gradient side by side in one buffer share no byte."""
+    buf = logits(torch, 9, 150, "bfloat16", 2)
+    x, out = buf[:, :64], buf[:, 70:134]
+    ids = torch.topk(x.float(), 4).indices.int()
+    dw = torch.rand(9, 4, device="cuda")
+    want = torch.empty_like(x, memory_format=torch.contiguous_format)
+    gpu.route_topk_backward(x, ids, dw, want, stream=0)
+    gpu.route_topk_backward(x, ids, dw, out, stream=0)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
