@@ -10,13 +10,16 @@
 // bits tell apart. The fast way computes in 32 bits and knows how far it may be off: it decides
 // alone where neighbours in the order stand further apart than that, orders the few doubtful
 // experts by their 64-bit values where not, and hands a token whose groups are in doubt to the
-// plain 64-bit way (which takes 70 us for the first case below, were it to do all of it).
+// plain 64-bit way (which takes 70 us for the first case below, were it to do all of it; a bias
+// of 6 for every expert, whose codes are all cut off, sends every token there by way of the fast
+// one: 103 us).
 //
 // What bounds it: instructions. A token of 256 experts, sigmoids, bias, 4 of 8 groups by their two
-// best, top-8, costs a warp 730; 16,384 of them as fp32 take 23 us, of which reading them is 3.
-// 32,768 tokens of 64 experts, softmax, top-6, bf16, all scores written: 9.5 us (14 MB, 2.2 at
-// HBM's rate). Their gradient 6.4 us (18 MB, 2.8); that of 10,007 tokens of the first kind, which
-// reads no logits but the chosen ones', 5.6 to 6.0 us (11 MB moved).
+// best, top-8, costs a warp 780; 16,384 of them as fp32 take 22.4 us, of which reading them is 3.
+// 32,768 tokens of 64 experts, softmax, top-6, bf16, all scores written: 9.3 us (14 MB, 2.2 at
+// HBM's rate). Their gradient 6.7 us (18 MB, 2.8); that of 10,007 tokens of the first kind, which
+// reads no logits but the chosen ones', 5.8 us (11 MB moved). 16,384 tokens of 512 and 1,024
+// experts, softmax, top-8, bf16: 15 and 24 us; 160 experts in 8 groups, the plain way: 52.
 #include "rows.cuh"
 
 #include "keys.cuh"

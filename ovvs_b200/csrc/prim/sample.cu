@@ -29,11 +29,11 @@
 //   - anything else: the edge of top-p is bracketed by a histogram of the weights over
 //     (m - x) / T, the few columns in the bracket are ordered by block 0, the weights above it
 //     are summed exactly. The draw walks the columns of the warp whose range of running sums
-//     holds it. 256 rows of 100,003 fp16, top-p 0.9, 11,000 columns kept: 157 us, 105 instructions
-//     for every 32 columns at 56 % of the issue rate, the rest waits of the cluster.
+//     holds it. 256 rows of 100,003 fp16, top-p 0.9, 11,000 columns kept: 162 us, 117 instructions
+//     for every 32 columns at 54 % of the issue rate, the rest waits of the cluster.
 // Where either meets more columns than its list holds (many equal or nearly equal scores), the
 // edge is found by parts of the range of score bits. 64 rows of 131,072 equal scores, top-p:
-// 390 us, against 104 for different ones.
+// 401 us, against 81 for different ones.
 #include "rows.cuh"
 
 #include <cooperative_groups.h>
@@ -570,8 +570,8 @@ __device__ void finish_list(const SampleParams& p, int64_t row, int n, const Set
 // left). A fifth block, for 48 registers, spills and brings nothing: 107 us with 38 KB, 134 with
 // 44; rows of that batch under top-p alone 905 us against 835.
 // Where a cluster takes a row, the weights want the registers: four of 64 in a large batch (256
-// rows of 100,003 fp16, top-p: 168 us, three of 80: 182, five of 48: 197), three of 80 in one that
-// leaves the SMs room (64 rows of 131,072 fp32, mixed: 54 us against 62). How many stand on an SM
+// rows of 100,003 fp16, top-p: 157 us, three of 80: 171), three of 80 in one that leaves the SMs
+// room (64 rows of 131,072 fp32, mixed: 57 us against 62). How many stand on an SM
 // is then often said by the part of the row that they hold: of that last case's blocks, 89 KB each,
 // two, so that 37 of its 64 clusters run at once. Three or four that hold less of it and read the
 // rest again take longer (67 us against 57).
@@ -1270,11 +1270,12 @@ cudaError_t sample(const SampleParams& p, cudaStream_t stream) {
   constexpr size_t kFixed = (sizeof(Shared) + 15) / 16 * 16;
   const int64_t chunks = (p.cols + 2 * kN - 2) / kN;  // whatever the row's alignment
   // A batch of two rows an SM or more that may have top-k rows goes one block a row, which reads a
-  // top-k row in one pass (512 rows of 100,003 fp16, top-50: 32 us against 86 by clusters of 8;
-  // rows under top-p alone, which it reads again from L2, take 354 against 296). Otherwise a row
-  // gets a cluster: up to three blocks an SM over all rows, of 512 chunks or more (16 rows of
-  // 32,000 bf16, top-p: 25 us by 8 blocks, 40 by 2), and beyond that as few as keep a block's
-  // part at 2048 chunks (400 such rows: 138 us by 8 blocks, 90 by 2, 112 by 1).
+  // top-k row in one pass (512 rows of 100,003 fp16, top-50: 28 us against 85 by clusters of 8;
+  // rows under top-p alone, which it reads again from L2, take 312 against 302, and a top-k above
+  // kDirectK takes four times as long as by clusters: 1000 rows of 100,000 fp32, top-1000, 3.9 ms).
+  // Otherwise a row gets a cluster: up to three blocks an SM over all rows, of 512 chunks or more
+  // (16 rows of 32,000 bf16, top-p: 25 us by 8 blocks, 41 by 2), and beyond that as few as keep a
+  // block's part at 2048 chunks (400 such rows: 140 us by 8 blocks, 97 by 4, 92 by 2, 117 by 1).
   const bool one_pass = p.top_k && p.rows >= 296;
   int nb = 1;
   while (nb < kMaxCluster && !one_pass && chunks / nb > 512 &&
