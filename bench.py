@@ -390,7 +390,7 @@ def _search_baseline(cfg, data_host, q_host, nb, ds, seconds):
         nb_ref, ds_ref = _oracle_sample(cfg, data_host, q_host, nq_s)
         baseline = {"value": None, "unavailable": missing}
         against = RESTATEMENT + "same queries"
-    # The same sampled queries' results from the timed runs, against the checker's.
+    # The same sampled queries' results from the timed runs, against theirs.
     parity = _parity(nb[:nq_s], ds[:nq_s], nb_ref, ds_ref,
                      2e-3 if cfg["dtype"] == "f16" else 1e-4)
     parity["against"] = against
